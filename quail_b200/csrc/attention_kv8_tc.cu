@@ -34,7 +34,7 @@
 // 128 t. O is rescaled only when a row's maximum grows by more than 2^8.
 // Registers: 128 a thread at launch, of which the loader's and the converters' warpgroups keep 88 and 72 and
 // the two softmax groups take 176: with 128 the scores spill (16k-token chunk 244 us, now 187; 4096 tokens
-// over 12k resident 1591 us, now 1325). The split is set inside each role's branch.
+// over 12k resident 1591 us, now 1325). One setmaxnreg a warpgroup, before its warps part into roles.
 // Every wait is bounded (common.cuh); on expiry a role records an error code
 // and stops, and the kernel drains its copies and MMAs before it frees TMEM.
 #include <torch/extension.h>
@@ -218,292 +218,295 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
+  // A warpgroup's registers are set by one setmaxnreg that all of its warps execute: under separate ones in the
+  // branches of its warps the instruction is undefined, and the raise to 176 waits for what the others give up.
+  if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    // ------------------------------------------------------------------ loader
-    const int pshift = __ffs(a.P) - 1, pmask = a.P - 1;
-    int it_raw = 0, idx = 0;
-    bool ok = true;
-    // (sequence, first token) of the items after this one, and the next one's row, are read ahead
-    auto block_of = [&](int item) -> int2 {
-      const int* b = a.blocks + 2 * (item / groups);
-      return item < n_items ? make_int2(b[0], b[1]) : make_int2(0, 0);
-    };
-    auto row_of = [&](int seq) -> const int* {
-      return a.seqs + (size_t)((unsigned)seq < (unsigned)a.n_seqs ? seq : 0) * kKv8SeqInts;
-    };
-    int2 b0 = block_of(blockIdx.x), b1 = block_of(blockIdx.x + gridDim.x);
-    Kv8Seq s;
-    kv8_load_seq(s, row_of(b0.x), 0);
-    for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++idx) {
-      const int q0 = b0.y;
-      const bool good = (unsigned)b0.x < (unsigned)a.n_seqs && q0 >= 0 && s.q_start >= 0 && s.q_len >= 0 &&
-                        s.q_start + s.q_len <= a.T;
-      if (!good && lane == 0) kv8_error(err, kErrBadShape);
-      Item it;
-      it.head0 = item % groups * 4;
-      const int kvh = it.head0 / (a.QH / a.KH);
-      const int left = good ? s.q_len - q0 : 0;
-      it.tok = s.q_start + q0;
-      it.rows_a = max(0, min(32, left));
-      it.rows_b = max(0, min(32, left - 32));
-      it.pos = s.own_len - s.q_len + q0;
-      it.n_a = it.n_b = it.pad = 0;
-      int before[kKv8MaxSeg], first[kKv8MaxSeg], cum[kKv8MaxSeg];      // keys and tiles before a segment
-      {
-        int base = 0, n = 0;
-#pragma unroll
-        for (int i = 0; i < kKv8MaxSeg; ++i) {
-          // the first row reaches furthest back, each tile's last row furthest ahead (earlier segments
-          // are seen alike, so only in the last one, the own, do the two tiles' ends differ)
-          int lo, hi, lo2, end_a, end_b;
-          kv8_span(s, i, s.len[i], base, it.pos, lo, hi);
-          kv8_span(s, i, s.len[i], base, it.pos + it.rows_a - 1, lo2, end_a);
-          kv8_span(s, i, s.len[i], base, it.pos + 31 + it.rows_b, lo2, end_b);
-          const bool there = i < s.nseg;
-          const int f = lo / kKeys;
-          const int e_a = there && it.rows_a > 0 && end_a > lo ? (end_a + kKeys - 1) / kKeys : f;
-          const int e_b = there && it.rows_b > 0 && end_b > lo ? (end_b + kKeys - 1) / kKeys : f;
-          before[i] = base;
-          first[i] = f;
-          cum[i] = n;
-          it.n_a += e_a - f;
-          it.n_b += e_b - f;
-          n += max(e_a, e_b) - f;
-          base += s.len[i];
-        }
-      }
-      const int nmax = max(it.n_a, it.n_b);
-      // the next item's row, and the block after it: not needed before this item's copies are issued
-      const int2 b2 = block_of(item + 2 * gridDim.x);
-      Kv8Seq next;
-      kv8_load_seq(next, row_of(b1.x), 0);
-      // 8 tiles at a time: lane 4 k + b looks up block b of tile k
-      struct Look {
-        uint32_t blk;
-        int bytes, x, y, z, blocks;
-      };
-      auto look = [&](int jb) -> Look {
-        Look r;
-        r.blk = 0;
-        r.bytes = 127 | 127 << 8;
-        r.blocks = 0;
-        const int j = jb + (lane >> 2);
-        int sg = 0;
-#pragma unroll
-        for (int i = 1; i < kKv8MaxSeg; ++i)
-          if (i < s.nseg && j >= cum[i]) sg = i;
-        int len = 0, off = 0, f = 0, base = 0, c = 0;
-#pragma unroll
-        for (int i = 0; i < kKv8MaxSeg; ++i)
-          if (i == sg) {
-            len = s.len[i];
-            off = s.off[i];
-            f = first[i];
-            base = before[i];
-            c = cum[i];
-          }
-        const int j0 = (f + j - c) * kKeys, key = j0 + (lane & 3) * 16, e = off + (key >> pshift);
-        const bool own = sg == s.nseg - 1;
-        // a row at own position p sees columns [p + z, min(x, p + y)) of the tile
-        r.x = len - j0;
-        r.y = own && !s.bidir ? 1 - j0 : 1 << 29;
-        r.z = s.win > 0 && (own ? !s.bidir : s.win_all) ? s.before - s.win + 1 - base - j0 : -(1 << 30);
-        if (j < nmax) {
-          r.blocks = min(4, (len - j0 + 15) / 16);       // 16-key blocks of the tile that exist
-          if ((lane & 3) < r.blocks) {
-            int page = (unsigned)e < (unsigned)a.n_list ? a.page_list[e] : -1;
-            if ((unsigned)page >= (unsigned)a.pages) {
-              kv8_error(err, kErrBadShape);
-              page = 0;
-            }
-            r.blk = ((uint32_t)(page * a.KH + kvh) << (pshift - 4)) + ((key & pmask) >> 4);
-            r.bytes = a.kb[r.blk] | (int)a.vb[r.blk] << 8;
-          }
-        }
-        return r;
-      };
-      Look cur = look(0);
-      if (lane == 0) {
-        const int sl = idx % kItems;
-        ok = mbar_wait(&item_empty[sl], (uint32_t)((idx / kItems) & 1) ^ 1, err, kErrTimeoutProducer);
-        if (ok) {
-          items[sl] = it;
-          mbar_arrive(&item_full[sl]);
-        }
-      }
-      ok = __shfl_sync(0xffffffffu, ok, 0);
-      for (int jb = 0; jb < nmax && ok; jb += 8) {
-        const Look then = look(jb + 8);
-        const int cnt = min(8, nmax - jb);
-        for (int k = 0; k < cnt && ok; ++k) {
-          const bool mine = (lane >> 2) == k;
-          const uint32_t k4 = __reduce_or_sync(0xffffffffu, mine ? (uint32_t)(cur.bytes & 0xff) << (8 * (lane & 3)) : 0u);
-          const uint32_t v4 = __reduce_or_sync(0xffffffffu, mine ? (uint32_t)(cur.bytes >> 8) << (8 * (lane & 3)) : 0u);
-          const int blocks = __shfl_sync(0xffffffffu, cur.blocks, 4 * k);
-          const int st = it_raw % kRaw;
-          if (mine && (lane & 3) == 0) {
-            ok = mbar_wait(&raw_empty[st], (uint32_t)((it_raw / kRaw) & 1) ^ 1, err, kErrTimeoutProducer);
-            if (ok) {
-              int* info = raw_info + 8 * st;
-              info[0] = (int)k4;
-              info[1] = (int)v4;
-              info[2] = cur.x;
-              info[3] = cur.y;
-              info[4] = cur.z;
-              mbar_arrive_expect_tx(&raw_full[st], 2 * blocks * 16 * kD);
-            }
-          }
-          ok = __shfl_sync(0xffffffffu, ok, 4 * k);
-          if (!ok) break;
-          uint8_t* dst = sRaw + st * kRawBytes + (lane & 3) * 16 * kD;
-          // in pages of 64 tokens and more a tile is one run of keys
-          if (mine && (lane & 3) < (a.P >= kKeys ? 1 : blocks)) {
-            const uint32_t bytes = (a.P >= kKeys ? blocks : 1) * 16 * kD;
-            bulk_load(dst, a.kc + (size_t)cur.blk * (16 * kD), bytes, &raw_full[st]);
-            bulk_load(dst + kKeys * kD, a.vc + (size_t)cur.blk * (16 * kD), bytes, &raw_full[st]);
-          }
-          ++it_raw;
-        }
-        cur = then;
-      }
-      s = next;
-      b0 = b1;
-      b1 = b2;
-    }
-    if (!ok && lane == 0) {
-      // stopped early: wait (bounded) for the copies already issued into shared memory
-      for (int k = max(0, it_raw - kRaw); k < it_raw; ++k)
-        mbar_wait(&raw_full[k % kRaw], (uint32_t)((k / kRaw) & 1), err, kErrTimeoutProducer);
-    }
-  } else if (warp == 1) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    // ------------------------------------------------------------------ MMA issuer
-    if (elect_one()) {
-      constexpr uint32_t IS = idesc_bf16(128, kKeys, 0);
-      constexpr uint32_t IO = idesc_bf16(128, kD, 1);
-      const uint32_t q_lo = (smem_u32(sQ) >> 4) | kLeadK, kv_lo = (smem_u32(sKV) >> 4) | kLeadK,
-                     p_lo = (smem_u32(sP) >> 4) | kLeadK;
-      int kv_base = 0, q_it = 0, idx = 0;
-      int s_cnt[2] = {0, 0}, p_cnt[2] = {0, 0}, free_cnt[2] = {0, 0};
-      bool had[2] = {false, false};
+    if (warp == 0) {
+      // ------------------------------------------------------------------ loader
+      const int pshift = __ffs(a.P) - 1, pmask = a.P - 1;
+      int it_raw = 0, idx = 0;
       bool ok = true;
-      auto kv_ready = [&](int j) -> bool {
-        const int st = (kv_base + j) % kStages;
-        if (!mbar_wait(&kv_full[st], (uint32_t)(((kv_base + j) / kStages) & 1), err, kErrTimeoutMma)) return false;
-        tc_fence_after();
-        return true;
+      // (sequence, first token) of the items after this one, and the next one's row, are read ahead
+      auto block_of = [&](int item) -> int2 {
+        const int* b = a.blocks + 2 * (item / groups);
+        return item < n_items ? make_int2(b[0], b[1]) : make_int2(0, 0);
       };
-      auto issue_s = [&](int t, int j) {
-        const uint32_t qa = q_lo + t * (kQBytes >> 4);
-        const uint32_t kb = kv_lo + (uint32_t)((kv_base + j) % kStages) * (2 * kTileBytes >> 4);
-        const uint32_t d = tmem + (uint32_t)((2 * t + (s_cnt[t] & 1)) * 64);
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks)
-          umma(d, qa + (ks >> 2) * (kRows * 128 >> 4) + (ks & 3) * 2, kb + (ks >> 2) * (kKeys * 128 >> 4) + (ks & 3) * 2,
-               IS, ks > 0 ? 1u : 0u);
-        tc_commit(&s_full[2 * t + (s_cnt[t] & 1)]);
-        ++s_cnt[t];
+      auto row_of = [&](int seq) -> const int* {
+        return a.seqs + (size_t)((unsigned)seq < (unsigned)a.n_seqs ? seq : 0) * kKv8SeqInts;
       };
-      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
-        const int sl = idx % kItems;
-        if (!mbar_wait(&item_full[sl], (uint32_t)((idx / kItems) & 1), err, kErrTimeoutMma)) {
-          ok = false;
-          break;
-        }
-        ++idx;
-        const int nt[2] = {items[sl].n_a, items[sl].n_b};
-        mbar_arrive(&item_empty[sl]);
-        const int nmax = max(nt[0], nt[1]);
-        if (nmax == 0) continue;
-        if (!mbar_wait(q_full, (uint32_t)(q_it & 1), err, kErrTimeoutMma)) {
-          ok = false;
-          break;
-        }
-        ++q_it;
-        tc_fence_after();
-        ok = kv_ready(0);
-        if (!ok) break;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-          if (nt[t] > 0) issue_s(t, 0);
-        if (nmax == 1) tc_commit(q_empty);
-        for (int j = 0; j < nmax && ok; ++j) {
-          if (j + 1 < nmax) {
-            // the other S buffer was read before P(j - 1) was handed over
-            ok = kv_ready(j + 1);
-            if (!ok) break;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-              if (j + 1 < nt[t]) issue_s(t, j + 1);
-            if (j + 2 == nmax) tc_commit(q_empty);
+      int2 b0 = block_of(blockIdx.x), b1 = block_of(blockIdx.x + gridDim.x);
+      Kv8Seq s;
+      kv8_load_seq(s, row_of(b0.x), 0);
+      for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++idx) {
+        const int q0 = b0.y;
+        const bool good = (unsigned)b0.x < (unsigned)a.n_seqs && q0 >= 0 && s.q_start >= 0 && s.q_len >= 0 &&
+                          s.q_start + s.q_len <= a.T;
+        if (!good && lane == 0) kv8_error(err, kErrBadShape);
+        Item it;
+        it.head0 = item % groups * 4;
+        const int kvh = it.head0 / (a.QH / a.KH);
+        const int left = good ? s.q_len - q0 : 0;
+        it.tok = s.q_start + q0;
+        it.rows_a = max(0, min(32, left));
+        it.rows_b = max(0, min(32, left - 32));
+        it.pos = s.own_len - s.q_len + q0;
+        it.n_a = it.n_b = it.pad = 0;
+        int before[kKv8MaxSeg], first[kKv8MaxSeg], cum[kKv8MaxSeg];      // keys and tiles before a segment
+        {
+          int base = 0, n = 0;
+  #pragma unroll
+          for (int i = 0; i < kKv8MaxSeg; ++i) {
+            // the first row reaches furthest back, each tile's last row furthest ahead (earlier segments
+            // are seen alike, so only in the last one, the own, do the two tiles' ends differ)
+            int lo, hi, lo2, end_a, end_b;
+            kv8_span(s, i, s.len[i], base, it.pos, lo, hi);
+            kv8_span(s, i, s.len[i], base, it.pos + it.rows_a - 1, lo2, end_a);
+            kv8_span(s, i, s.len[i], base, it.pos + 31 + it.rows_b, lo2, end_b);
+            const bool there = i < s.nseg;
+            const int f = lo / kKeys;
+            const int e_a = there && it.rows_a > 0 && end_a > lo ? (end_a + kKeys - 1) / kKeys : f;
+            const int e_b = there && it.rows_b > 0 && end_b > lo ? (end_b + kKeys - 1) / kKeys : f;
+            before[i] = base;
+            first[i] = f;
+            cum[i] = n;
+            it.n_a += e_a - f;
+            it.n_b += e_b - f;
+            n += max(e_a, e_b) - f;
+            base += s.len[i];
           }
-          const int st = (kv_base + j) % kStages;
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (j >= nt[t] || !ok) continue;
-            if (!mbar_wait(&p_full[t], (uint32_t)(p_cnt[t] & 1), err, kErrTimeoutMma)) {
-              ok = false;
-              continue;
+        }
+        const int nmax = max(it.n_a, it.n_b);
+        // the next item's row, and the block after it: not needed before this item's copies are issued
+        const int2 b2 = block_of(item + 2 * gridDim.x);
+        Kv8Seq next;
+        kv8_load_seq(next, row_of(b1.x), 0);
+        // 8 tiles at a time: lane 4 k + b looks up block b of tile k
+        struct Look {
+          uint32_t blk;
+          int bytes, x, y, z, blocks;
+        };
+        auto look = [&](int jb) -> Look {
+          Look r;
+          r.blk = 0;
+          r.bytes = 127 | 127 << 8;
+          r.blocks = 0;
+          const int j = jb + (lane >> 2);
+          int sg = 0;
+  #pragma unroll
+          for (int i = 1; i < kKv8MaxSeg; ++i)
+            if (i < s.nseg && j >= cum[i]) sg = i;
+          int len = 0, off = 0, f = 0, base = 0, c = 0;
+  #pragma unroll
+          for (int i = 0; i < kKv8MaxSeg; ++i)
+            if (i == sg) {
+              len = s.len[i];
+              off = s.off[i];
+              f = first[i];
+              base = before[i];
+              c = cum[i];
             }
-            ++p_cnt[t];
-            if (j == 0 && had[t]) {
-              // the previous item's epilogue has read O_t out of TMEM
-              if (!mbar_wait(&o_free[t], (uint32_t)(free_cnt[t] & 1), err, kErrTimeoutMma)) {
+          const int j0 = (f + j - c) * kKeys, key = j0 + (lane & 3) * 16, e = off + (key >> pshift);
+          const bool own = sg == s.nseg - 1;
+          // a row at own position p sees columns [p + z, min(x, p + y)) of the tile
+          r.x = len - j0;
+          r.y = own && !s.bidir ? 1 - j0 : 1 << 29;
+          r.z = s.win > 0 && (own ? !s.bidir : s.win_all) ? s.before - s.win + 1 - base - j0 : -(1 << 30);
+          if (j < nmax) {
+            r.blocks = min(4, (len - j0 + 15) / 16);       // 16-key blocks of the tile that exist
+            if ((lane & 3) < r.blocks) {
+              int page = (unsigned)e < (unsigned)a.n_list ? a.page_list[e] : -1;
+              if ((unsigned)page >= (unsigned)a.pages) {
+                kv8_error(err, kErrBadShape);
+                page = 0;
+              }
+              r.blk = ((uint32_t)(page * a.KH + kvh) << (pshift - 4)) + ((key & pmask) >> 4);
+              r.bytes = a.kb[r.blk] | (int)a.vb[r.blk] << 8;
+            }
+          }
+          return r;
+        };
+        Look cur = look(0);
+        if (lane == 0) {
+          const int sl = idx % kItems;
+          ok = mbar_wait(&item_empty[sl], (uint32_t)((idx / kItems) & 1) ^ 1, err, kErrTimeoutProducer);
+          if (ok) {
+            items[sl] = it;
+            mbar_arrive(&item_full[sl]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+        for (int jb = 0; jb < nmax && ok; jb += 8) {
+          const Look then = look(jb + 8);
+          const int cnt = min(8, nmax - jb);
+          for (int k = 0; k < cnt && ok; ++k) {
+            const bool mine = (lane >> 2) == k;
+            const int at8 = 8 * (lane & 3);
+            const uint32_t k4 = __reduce_or_sync(0xffffffffu, mine ? (uint32_t)(cur.bytes & 0xff) << at8 : 0u);
+            const uint32_t v4 = __reduce_or_sync(0xffffffffu, mine ? (uint32_t)(cur.bytes >> 8) << at8 : 0u);
+            const int blocks = __shfl_sync(0xffffffffu, cur.blocks, 4 * k);
+            const int st = it_raw % kRaw;
+            if (mine && (lane & 3) == 0) {
+              ok = mbar_wait(&raw_empty[st], (uint32_t)((it_raw / kRaw) & 1) ^ 1, err, kErrTimeoutProducer);
+              if (ok) {
+                int* info = raw_info + 8 * st;
+                info[0] = (int)k4;
+                info[1] = (int)v4;
+                info[2] = cur.x;
+                info[3] = cur.y;
+                info[4] = cur.z;
+                mbar_arrive_expect_tx(&raw_full[st], 2 * blocks * 16 * kD);
+              }
+            }
+            ok = __shfl_sync(0xffffffffu, ok, 4 * k);
+            if (!ok) break;
+            uint8_t* dst = sRaw + st * kRawBytes + (lane & 3) * 16 * kD;
+            // in pages of 64 tokens and more a tile is one run of keys
+            if (mine && (lane & 3) < (a.P >= kKeys ? 1 : blocks)) {
+              const uint32_t bytes = (a.P >= kKeys ? blocks : 1) * 16 * kD;
+              bulk_load(dst, a.kc + (size_t)cur.blk * (16 * kD), bytes, &raw_full[st]);
+              bulk_load(dst + kKeys * kD, a.vc + (size_t)cur.blk * (16 * kD), bytes, &raw_full[st]);
+            }
+            ++it_raw;
+          }
+          cur = then;
+        }
+        s = next;
+        b0 = b1;
+        b1 = b2;
+      }
+      if (!ok && lane == 0) {
+        // stopped early: wait (bounded) for the copies already issued into shared memory
+        for (int k = max(0, it_raw - kRaw); k < it_raw; ++k)
+          mbar_wait(&raw_full[k % kRaw], (uint32_t)((k / kRaw) & 1), err, kErrTimeoutProducer);
+      }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------------ MMA issuer
+      if (elect_one()) {
+        constexpr uint32_t IS = idesc_bf16(128, kKeys, 0);
+        constexpr uint32_t IO = idesc_bf16(128, kD, 1);
+        const uint32_t q_lo = (smem_u32(sQ) >> 4) | kLeadK, kv_lo = (smem_u32(sKV) >> 4) | kLeadK,
+                       p_lo = (smem_u32(sP) >> 4) | kLeadK;
+        int kv_base = 0, q_it = 0, idx = 0;
+        int s_cnt[2] = {0, 0}, p_cnt[2] = {0, 0}, free_cnt[2] = {0, 0};
+        bool had[2] = {false, false};
+        bool ok = true;
+        auto kv_ready = [&](int j) -> bool {
+          const int st = (kv_base + j) % kStages;
+          if (!mbar_wait(&kv_full[st], (uint32_t)(((kv_base + j) / kStages) & 1), err, kErrTimeoutMma)) return false;
+          tc_fence_after();
+          return true;
+        };
+        auto issue_s = [&](int t, int j) {
+          const uint32_t qa = q_lo + t * (kQBytes >> 4);
+          const uint32_t kb = kv_lo + (uint32_t)((kv_base + j) % kStages) * (2 * kTileBytes >> 4);
+          const uint32_t d = tmem + (uint32_t)((2 * t + (s_cnt[t] & 1)) * 64);
+  #pragma unroll
+          for (int ks = 0; ks < 8; ++ks)
+            umma(d, qa + (ks >> 2) * (kRows * 128 >> 4) + (ks & 3) * 2,
+                 kb + (ks >> 2) * (kKeys * 128 >> 4) + (ks & 3) * 2, IS, ks > 0 ? 1u : 0u);
+          tc_commit(&s_full[2 * t + (s_cnt[t] & 1)]);
+          ++s_cnt[t];
+        };
+        for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x) {
+          const int sl = idx % kItems;
+          if (!mbar_wait(&item_full[sl], (uint32_t)((idx / kItems) & 1), err, kErrTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          ++idx;
+          const int nt[2] = {items[sl].n_a, items[sl].n_b};
+          mbar_arrive(&item_empty[sl]);
+          const int nmax = max(nt[0], nt[1]);
+          if (nmax == 0) continue;
+          if (!mbar_wait(q_full, (uint32_t)(q_it & 1), err, kErrTimeoutMma)) {
+            ok = false;
+            break;
+          }
+          ++q_it;
+          tc_fence_after();
+          ok = kv_ready(0);
+          if (!ok) break;
+  #pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (nt[t] > 0) issue_s(t, 0);
+          if (nmax == 1) tc_commit(q_empty);
+          for (int j = 0; j < nmax && ok; ++j) {
+            if (j + 1 < nmax) {
+              // the other S buffer was read before P(j - 1) was handed over
+              ok = kv_ready(j + 1);
+              if (!ok) break;
+  #pragma unroll
+              for (int t = 0; t < 2; ++t)
+                if (j + 1 < nt[t]) issue_s(t, j + 1);
+              if (j + 2 == nmax) tc_commit(q_empty);
+            }
+            const int st = (kv_base + j) % kStages;
+  #pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (j >= nt[t] || !ok) continue;
+              if (!mbar_wait(&p_full[t], (uint32_t)(p_cnt[t] & 1), err, kErrTimeoutMma)) {
                 ok = false;
                 continue;
               }
-              ++free_cnt[t];
+              ++p_cnt[t];
+              if (j == 0 && had[t]) {
+                // the previous item's epilogue has read O_t out of TMEM
+                if (!mbar_wait(&o_free[t], (uint32_t)(free_cnt[t] & 1), err, kErrTimeoutMma)) {
+                  ok = false;
+                  continue;
+                }
+                ++free_cnt[t];
+              }
+              tc_fence_after();
+              const uint32_t pa = p_lo + t * (kPBytes >> 4);
+              const uint32_t vb = kv_lo + (uint32_t)st * (2 * kTileBytes >> 4) + (kTileBytes >> 4) + (kLeadV - kLeadK);
+  #pragma unroll
+              for (int ks = 0; ks < 4; ++ks)
+                umma(tmem + 256u + (uint32_t)(t * 128), pa + ks * 2, vb + ks * (16 * 128 >> 4), IO,
+                     (j > 0 || ks > 0) ? 1u : 0u);
+              tc_commit(&o_done[t]);
             }
-            tc_fence_after();
-            const uint32_t pa = p_lo + t * (kPBytes >> 4);
-            const uint32_t vb = kv_lo + (uint32_t)st * (2 * kTileBytes >> 4) + (kTileBytes >> 4) + (kLeadV - kLeadK);
-#pragma unroll
-            for (int ks = 0; ks < 4; ++ks)
-              umma(tmem + 256u + (uint32_t)(t * 128), pa + ks * 2, vb + ks * (16 * 128 >> 4), IO,
-                   (j > 0 || ks > 0) ? 1u : 0u);
-            tc_commit(&o_done[t]);
+            if (ok) tc_commit(&kv_empty[st]);
           }
-          if (ok) tc_commit(&kv_empty[st]);
+          if (!ok) break;
+          had[0] = had[0] || nt[0] > 0;
+          had[1] = had[1] || nt[1] > 0;
+          kv_base += nmax;
         }
-        if (!ok) break;
-        had[0] = had[0] || nt[0] > 0;
-        had[1] = had[1] || nt[1] > 0;
-        kv_base += nmax;
+        tc_commit(mma_idle);
+        mbar_wait(mma_idle, 0, err, kErrTimeoutMma);
       }
-      tc_commit(mma_idle);
-      mbar_wait(mma_idle, 0, err, kErrTimeoutMma);
-    }
-  } else if (warp == 2) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    // ------------------------------------------------------------------ Q
-    if (lane == 0) {
-      tma_prefetch_desc(&tmQ);
-      int q_it = 0, idx = 0;
-      bool ok = true;
-      for (int item = blockIdx.x; item < n_items; item += gridDim.x, ++idx) {
-        const int sl = idx % kItems;
-        ok = mbar_wait_idle(&item_full[sl], (uint32_t)((idx / kItems) & 1), err, kErrTimeoutProducer, 200);
-        if (!ok) break;
-        const int tok = items[sl].tok, head0 = items[sl].head0;
-        const bool any = max(items[sl].n_a, items[sl].n_b) > 0;
-        mbar_arrive(&item_empty[sl]);
-        if (!any) continue;
-        tma_prefetch_3d(&tmQ, 0, head0, tok);
-        tma_prefetch_3d(&tmQ, 64, head0, tok);
-        tma_prefetch_3d(&tmQ, 0, head0, tok + 32);
-        tma_prefetch_3d(&tmQ, 64, head0, tok + 32);
-        ok = mbar_wait_idle(q_empty, (uint32_t)((q_it & 1) ^ 1), err, kErrTimeoutProducer, 100);
-        if (!ok) break;
-        mbar_arrive_expect_tx(q_full, 2 * kQBytes);
-        tma_load_3d(&tmQ, q_full, sQ, 0, head0, tok);
-        tma_load_3d(&tmQ, q_full, sQ + kQBytes / 2, 64, head0, tok);
-        tma_load_3d(&tmQ, q_full, sQ + kQBytes, 0, head0, tok + 32);
-        tma_load_3d(&tmQ, q_full, sQ + kQBytes + kQBytes / 2, 64, head0, tok + 32);
-        ++q_it;
+    } else if (warp == 2) {
+      // ------------------------------------------------------------------ Q
+      if (lane == 0) {
+        tma_prefetch_desc(&tmQ);
+        int q_it = 0, idx = 0;
+        bool ok = true;
+        for (int item = blockIdx.x; item < n_items; item += gridDim.x, ++idx) {
+          const int sl = idx % kItems;
+          ok = mbar_wait_idle(&item_full[sl], (uint32_t)((idx / kItems) & 1), err, kErrTimeoutProducer, 200);
+          if (!ok) break;
+          const int tok = items[sl].tok, head0 = items[sl].head0;
+          const bool any = max(items[sl].n_a, items[sl].n_b) > 0;
+          mbar_arrive(&item_empty[sl]);
+          if (!any) continue;
+          tma_prefetch_3d(&tmQ, 0, head0, tok);
+          tma_prefetch_3d(&tmQ, 64, head0, tok);
+          tma_prefetch_3d(&tmQ, 0, head0, tok + 32);
+          tma_prefetch_3d(&tmQ, 64, head0, tok + 32);
+          ok = mbar_wait_idle(q_empty, (uint32_t)((q_it & 1) ^ 1), err, kErrTimeoutProducer, 100);
+          if (!ok) break;
+          mbar_arrive_expect_tx(q_full, 2 * kQBytes);
+          tma_load_3d(&tmQ, q_full, sQ, 0, head0, tok);
+          tma_load_3d(&tmQ, q_full, sQ + kQBytes / 2, 64, head0, tok);
+          tma_load_3d(&tmQ, q_full, sQ + kQBytes, 0, head0, tok + 32);
+          tma_load_3d(&tmQ, q_full, sQ + kQBytes + kQBytes / 2, 64, head0, tok + 32);
+          ++q_it;
+        }
+        // stopped early: wait (bounded) for the copies already issued into shared memory
+        if (!ok && q_it > 0) mbar_wait(q_full, (uint32_t)((q_it - 1) & 1), err, kErrTimeoutProducer);
       }
-      // stopped early: wait (bounded) for the copies already issued into shared memory
-      if (!ok && q_it > 0) mbar_wait(q_full, (uint32_t)((q_it - 1) & 1), err, kErrTimeoutProducer);
     }
   } else if (warp >= 12) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
@@ -562,11 +565,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_arrive(&raw_empty[rs]);
       }
     }
-  } else if (warp == 3) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
   } else {
-    // ------------------------------------------------------------------ softmax + epilogue
     asm volatile("setmaxnreg.inc.sync.aligned.u32 176;");
+    // ------------------------------------------------------------------ softmax + epilogue
     const int t = (warp - 4) >> 2;                      // tile A (warps 4-7) or B (warps 8-11)
     const int quarter = warp & 3;                       // TMEM lane quarter this warp may access
     const int row = quarter * 32 + lane;
