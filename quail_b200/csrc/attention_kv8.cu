@@ -358,7 +358,9 @@ Kv8Attn kv8_args(const char* what, const torch::Tensor& q, const torch::Tensor& 
               ": q [T, QH, D] bf16 beside the pages");
   const int64_t T = q.size(0), QH = q.size(1), D = q.size(2), KH = kc.size(1);
   TORCH_CHECK(D == kc.size(3) && (D == 64 || D == 128 || D == 256), what, ": head_dim 64, 128 or 256, as the pages'");
-  TORCH_CHECK(QH % KH == 0, what, ": q heads must be a multiple of KV heads");
+  TORCH_CHECK(KH > 0 && QH > 0 && QH % KH == 0, what, ": q heads must be a multiple of KV heads");
+  // where a page number is out of range the kernels report it and read page 0 instead
+  TORCH_CHECK(kc.size(0) > 0, what, ": at least one page");
   TORCH_CHECK(seqs.dim() == 2 && seqs.size(1) == kKv8SeqInts && seqs.scalar_type() == at::kInt &&
                   seqs.is_contiguous() && seqs.device() == q.device() && seqs.size(0) > 0,
               what, ": seqs [S, 12] int32, at least one");

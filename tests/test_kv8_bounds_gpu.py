@@ -1,0 +1,42 @@
+"""What the 8-bit KV operators refuse or report because a kernel would otherwise read or write out of range."""
+
+import pytest
+import torch
+
+from quail_b200 import ops
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda"
+I32 = dict(dtype=torch.int32, device=DEV)
+GEOMETRIES = [(8, 2, 128), (4, 2, 128), (4, 1, 256)]      # tcgen05 and mma.sync prefill
+
+
+@pytest.fixture(autouse=True)
+def _no_kernel_errors():
+    torch.manual_seed(0)
+    yield
+    assert ops.read_and_clear_error(0) == 0
+
+
+def one_sequence(QH, KH, D, pages=4, P=16, tokens=6, length=20, kind="int8"):
+    kp, vp = (ops.Pages8.zeros(pages, P, KH, D, ops.KV8_DTYPES[kind], DEV) for _ in range(2))
+    q = torch.randn(tokens, QH, D, device=DEV).bfloat16()
+    seqs = torch.tensor([[0, tokens, 1, 0, length, 0, 0, 0, 0, 0, 0, 0]], **I32)
+    return q, kp, vp, seqs, torch.zeros(1, 2, **I32), torch.arange(-(-length // P), **I32)
+
+
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+def test_a_cache_without_pages_is_refused(QH, KH, D):
+    # a key whose page is out of range is reported and page 0 read instead: there has to be one
+    q, kp, vp, seqs, blocks, pl = one_sequence(QH, KH, D, pages=0)
+    with pytest.raises(RuntimeError, match="at least one page"):
+        ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1)
+    with pytest.raises(RuntimeError, match="at least one page"):
+        ops.decode_attention_kv8(q, kp, vp, seqs, torch.zeros(1, **I32), pl, 0.1)
+    # the write and the read report every slot of it
+    rows = torch.randn(2, KH, D, device=DEV).bfloat16()
+    ops.kv8_write(rows, rows, torch.tensor([0, 5], **I32), kp, vp)
+    assert ops.read_and_clear_error(0) == 5
+    k, v = ops.kv8_read(kp, vp, torch.tensor([0, 5], **I32))
+    assert ops.read_and_clear_error(0) == 5 and not bool(k.any()) and not bool(v.any())
