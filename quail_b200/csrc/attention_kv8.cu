@@ -395,6 +395,9 @@ Kv8Attn kv8_args(const char* what, const torch::Tensor& q, const torch::Tensor& 
     TORCH_CHECK(QH * D % 128 == 0 && out_sf.has_value() && out_sf->scalar_type() == at::kByte &&
                     out_sf->is_contiguous() && out_sf->numel() >= (T + 127) / 128 * (QH * D / 128) * 512,
                 what, ": e4m3 output needs its MX scale bytes");
+    // the tcgen05 prefill stores a row's four scale bytes as a word
+    TORCH_CHECK(out_sf->device() == q.device() && reinterpret_cast<uintptr_t>(out_sf->data_ptr()) % 4 == 0, what,
+                ": the MX scale bytes are 4-byte aligned and beside q");
     TORCH_CHECK(!lse.has_value(), what, ": a log-sum-exp output goes with a bf16 out");
     a.o8 = static_cast<uint8_t*>(out.data_ptr());
     a.osf = out_sf->data_ptr<uint8_t>();

@@ -40,3 +40,15 @@ def test_a_cache_without_pages_is_refused(QH, KH, D):
     assert ops.read_and_clear_error(0) == 5
     k, v = ops.kv8_read(kp, vp, torch.tensor([0, 5], **I32))
     assert ops.read_and_clear_error(0) == 5 and not bool(k.any()) and not bool(v.any())
+
+
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+def test_scale_bytes_elsewhere_or_unaligned_are_refused(QH, KH, D):
+    q, kp, vp, seqs, blocks, pl = one_sequence(QH, KH, D)
+    n = ops.sf_bytes(q.shape[0], QH * D)
+    dseqs = torch.zeros(1, **I32)
+    for sf in (torch.zeros(n, dtype=torch.uint8), torch.zeros(n + 1, dtype=torch.uint8, device=DEV)[1:]):
+        with pytest.raises(RuntimeError, match="scale bytes"):
+            ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1, fp8_out=True, out_scale=sf)
+        with pytest.raises(RuntimeError, match="scale bytes"):
+            ops.decode_attention_kv8(q, kp, vp, seqs, dseqs, pl, 0.1, fp8_out=True, out_scale=sf)
