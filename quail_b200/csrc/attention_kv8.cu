@@ -77,13 +77,13 @@ __global__ void __launch_bounds__(128) attn_kv8_kernel(const __grid_constant__ K
   Kv8Seq s;
   kv8_load_seq(s, a.seqs, seq);
   const int q0 = a.blocks[2 * blockIdx.x + 1];
-  const int tokens = min(64, s.q_len - q0);                // of the block
-  const int row0 = blockIdx.z * 64;                        // first of this CTA's rows in the block
-  if (row0 >= tokens * G || q0 < 0) return;
-  if (s.q_start < 0 || s.q_start + s.q_len > a.T) {
+  if (q0 < 0 || !kv8_rows_ok(s, a.T)) {
     if (tid == 0) kv8_error(a.err, kErrBadShape);
     return;
   }
+  const int tokens = min(64, s.q_len - q0);                // of the block
+  const int row0 = blockIdx.z * 64;                        // first of this CTA's rows in the block
+  if (row0 >= tokens * G) return;
   const int last_row = min(row0 + 64, tokens * G) - 1;
   const int shift = s.own_len - s.q_len + q0;              // own position of the block's first token
   const int pos_first = shift + row0 / G, pos_last = shift + last_row / G;

@@ -240,8 +240,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       kv8_load_seq(s, row_of(b0.x), 0);
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++idx) {
         const int q0 = b0.y;
-        const bool good = (unsigned)b0.x < (unsigned)a.n_seqs && q0 >= 0 && s.q_start >= 0 && s.q_len >= 0 &&
-                          s.q_start + s.q_len <= a.T;
+        const bool good = (unsigned)b0.x < (unsigned)a.n_seqs && q0 >= 0 && kv8_rows_ok(s, a.T);
         if (!good && lane == 0) kv8_error(err, kErrBadShape);
         Item it;
         it.head0 = item % groups * 4;

@@ -154,6 +154,11 @@ __device__ __forceinline__ void kv8_load_seq(Kv8Seq& s, const int* __restrict__ 
   }
 }
 
+// Whether a sequence's query rows are among the T there are (their sum may pass 32 bits).
+__device__ __forceinline__ bool kv8_rows_ok(const Kv8Seq& s, int T) {
+  return s.q_start >= 0 && s.q_len >= 0 && s.q_len <= T - s.q_start;
+}
+
 // Keys [lo, hi) of segment `seg` (with `base` keys before it) that a query at
 // own-segment position `pos` sees.
 __device__ __forceinline__ void kv8_span(const Kv8Seq& s, int seg, int seg_len, int base, int pos, int& lo, int& hi) {

@@ -52,3 +52,27 @@ def test_scale_bytes_elsewhere_or_unaligned_are_refused(QH, KH, D):
             ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1, fp8_out=True, out_scale=sf)
         with pytest.raises(RuntimeError, match="scale bytes"):
             ops.decode_attention_kv8(q, kp, vp, seqs, dseqs, pl, 0.1, fp8_out=True, out_scale=sf)
+
+
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+@pytest.mark.parametrize("start,count", [(2 ** 31 - 4, 6), (1, 2 ** 31 - 1), (2 ** 31 - 1, 2 ** 31 - 1), (3, 6), (-1, 6),
+                                         (0, -2 ** 31), (7, 0)])
+def test_query_rows_out_of_range_are_reported(QH, KH, D, start, count):
+    # also where first row + rows is past 32 bits
+    q, kp, vp, seqs, blocks, pl = one_sequence(QH, KH, D)
+    seqs[0, 0], seqs[0, 1] = start, count
+    out = torch.full((q.shape[0], QH * D), 7.0, dtype=torch.bfloat16, device=DEV)
+    ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1, out=out)
+    assert ops.read_and_clear_error(0) == 5 and bool((out == 7).all())
+    if count > 0:
+        ops.decode_attention_kv8(q, kp, vp, seqs, torch.zeros(1, **I32), pl, 0.1, out=out)
+        assert ops.read_and_clear_error(0) == 5 and bool((out == 7).all())
+
+
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+def test_a_block_before_its_sequence_is_reported(QH, KH, D):
+    q, kp, vp, seqs, blocks, pl = one_sequence(QH, KH, D)
+    out = torch.full((q.shape[0], QH * D), 7.0, dtype=torch.bfloat16, device=DEV)
+    blocks[0, 1] = -64
+    ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1, out=out)
+    assert ops.read_and_clear_error(0) == 5 and bool((out == 7).all())
