@@ -75,7 +75,7 @@ __global__ void __launch_bounds__(128) attn_kv8_kernel(const __grid_constant__ K
     return;
   }
   Kv8Seq s;
-  kv8_load_seq(s, a.seqs, seq);
+  kv8_load_seq(s, a, seq);
   const int q0 = a.blocks[2 * blockIdx.x + 1];
   if (q0 < 0 || !kv8_rows_ok(s, a.T)) {
     if (tid == 0) kv8_error(a.err, kErrBadShape);
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(128) attn_kv8_kernel(const __grid_constant__ K
       rk[c] = rv[c] = make_uint4(0, 0, 0, 0);
       if (j < len) {
         const int e = off + (j >> pshift);
-        const int page = (unsigned)e < (unsigned)a.n_list ? a.page_list[e] : -1;
+        const int page = a.page_list[e];
         if ((unsigned)page < (unsigned)a.pages) {
           const size_t at = (((size_t)page * a.KH + kvh) * a.P + (j & pmask)) * D + col * 16;
           rk[c] = *reinterpret_cast<const uint4*>(a.kc + at);
@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(128) attn_kv8_kernel(const __grid_constant__ K
     if (tid < 2 * (BK / 16)) {
       const int j = tile * BK + (tid % (BK / 16)) * 16;
       const int e = off + (j >> pshift);
-      if (j < len && (unsigned)e < (unsigned)a.n_list) {
+      if (j < len) {
         const int page = a.page_list[e];
         if ((unsigned)page < (unsigned)a.pages)
           rbyte = (tid < BK / 16 ? a.kb : a.vb)[((size_t)page * a.KH + kvh) * (a.P / 16) + ((j & pmask) >> 4)];
@@ -371,6 +371,8 @@ Kv8Attn kv8_args(const char* what, const torch::Tensor& q, const torch::Tensor& 
   TORCH_CHECK(out.dim() == 2 && out.size(0) == T && out.size(1) == QH * D && out.is_contiguous() &&
                   out.device() == q.device(),
               what, ": out [T, QH*D]");
+  // the kernels sum a sequence's (at most 4) segments, none longer than the list, in 32 bits
+  TORCH_CHECK(page_list.numel() <= INT32_MAX / kKv8MaxSeg / kc.size(2), what, ": the page list passes 2^29 tokens");
   Kv8Attn a;
   a.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
   a.kc = static_cast<const uint8_t*>(kc.data_ptr());

@@ -150,7 +150,7 @@ __device__ __forceinline__ int seq_row(const Kv8Attn& a, const Kv8Seq& s) {
 __device__ __forceinline__ bool load_dseq(const Kv8Attn& a, int i, Kv8Seq& s) {
   const int seq = a.blocks[i];
   if ((unsigned)seq < (unsigned)a.n_seqs) {
-    kv8_load_seq(s, a.seqs, seq);
+    kv8_load_seq(s, a, seq);
     return true;
   }
   kv8_error(a.err, kErrBadShape);
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(DecGeom<D>::kWarps * 32, DecGeom<D>::kBlocksPe
     for (int h = 0; h < (SMALL ? 2 : 1); ++h) {
       const int j = ptile * kTile + h * 16, e = ps.x + (j >> pshift);
       page[h] = 0;
-      if (j < ps.z) page[h] = (unsigned)e < (unsigned)a.n_list ? a.page_list[e] : a.pages;
+      if (j < ps.z) page[h] = a.page_list[e];
     }
   };
   uint32_t blk[2] = {0, 0};                                                // the cursor's blocks of 16 keys
@@ -933,8 +933,11 @@ void decode_attention_kv8(const torch::Tensor& q, const torch::Tensor& kc, const
   cudaStream_t st = at::cuda::getCurrentCUDAStream(dev);
   const bool fp8 = kc.scalar_type() == at::kFloat8_e4m3fn, mx = a.o8 != nullptr;
   const int D = (int)q.size(2);
-  for (int first = 0; first < total; first += kMaxRows) {
-    const int n = std::min(kMaxRows, total - first);
+  // the tiles of a launch are counted in 32 bits: a row has at most 4 times the page list's
+  const int64_t row_tiles = kKv8MaxSeg * ((int64_t)a.n_list * a.P / kTile + 1);
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxRows, INT32_MAX / row_tiles));
+  for (int first = 0; first < total; first += most) {
+    const int n = std::min(most, total - first);
     a.blocks = dseqs.data_ptr<int>() + first;
 #define QB_DEC8(DD)                                                                                     \
   if (D == DD) {                                                                                        \

@@ -232,12 +232,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int* b = a.blocks + 2 * (item / groups);
         return item < n_items ? make_int2(b[0], b[1]) : make_int2(0, 0);
       };
-      auto row_of = [&](int seq) -> const int* {
-        return a.seqs + (size_t)((unsigned)seq < (unsigned)a.n_seqs ? seq : 0) * kKv8SeqInts;
-      };
+      auto row_of = [&](int seq) { return (unsigned)seq < (unsigned)a.n_seqs ? seq : 0; };
       int2 b0 = block_of(blockIdx.x), b1 = block_of(blockIdx.x + gridDim.x);
       Kv8Seq s;
-      kv8_load_seq(s, row_of(b0.x), 0);
+      kv8_load_seq(s, a, row_of(b0.x));
       for (int item = blockIdx.x; item < n_items && ok; item += gridDim.x, ++idx) {
         const int q0 = b0.y;
         const bool good = (unsigned)b0.x < (unsigned)a.n_seqs && q0 >= 0 && kv8_rows_ok(s, a.T);
@@ -279,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the next item's row, and the block after it: not needed before this item's copies are issued
         const int2 b2 = block_of(item + 2 * gridDim.x);
         Kv8Seq next;
-        kv8_load_seq(next, row_of(b1.x), 0);
+        kv8_load_seq(next, a, row_of(b1.x));
         // 8 tiles at a time: lane 4 k + b looks up block b of tile k
         struct Look {
           uint32_t blk;
@@ -314,7 +312,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j < nmax) {
             r.blocks = min(4, (len - j0 + 15) / 16);       // 16-key blocks of the tile that exist
             if ((lane & 3) < r.blocks) {
-              int page = (unsigned)e < (unsigned)a.n_list ? a.page_list[e] : -1;
+              int page = a.page_list[e];
               if ((unsigned)page >= (unsigned)a.pages) {
                 kv8_error(err, kErrBadShape);
                 page = 0;

@@ -128,8 +128,10 @@ struct Kv8Seq {
   int len[kKv8MaxSeg], off[kKv8MaxSeg];
 };
 
-__device__ __forceinline__ void kv8_load_seq(Kv8Seq& s, const int* __restrict__ seqs, int seq) {
-  const int* sd = seqs + (size_t)seq * kKv8SeqInts;      // a view of a packed buffer: 4-byte aligned
+// Segments that reach past the page list are reported and count as empty, so that every key's place in the list is
+// inside it, and the sums of a table's lengths (which the host bounds by the list's) stay in 32 bits.
+__device__ __forceinline__ void kv8_load_seq(Kv8Seq& s, const Kv8Attn& a, int seq) {
+  const int* sd = a.seqs + (size_t)seq * kKv8SeqInts;    // a view of a packed buffer: 4-byte aligned
   int v[kKv8SeqInts];
 #pragma unroll
   for (int i = 0; i < kKv8SeqInts; ++i) v[i] = __ldg(sd + i);
@@ -139,16 +141,20 @@ __device__ __forceinline__ void kv8_load_seq(Kv8Seq& s, const int* __restrict__ 
   s.bidir = (v[3] & 1) != 0;
   s.win = (v[3] >> 8) & 0xffff;
   s.win_all = (v[3] >> 24) & 1;
+  const int pshift = __ffs(a.P) - 1;
 #pragma unroll
   for (int i = 0; i < kKv8MaxSeg; ++i) {
-    s.len[i] = i < s.nseg ? v[4 + i] : 0;
+    s.len[i] = i < s.nseg ? max(v[4 + i], 0) : 0;
     s.off[i] = v[4 + kKv8MaxSeg + i];
+    if (s.len[i] > 0 && (s.off[i] < 0 || (s.len[i] - 1) >> pshift >= a.n_list - s.off[i])) {
+      kv8_error(a.err, kErrBadShape);
+      s.len[i] = 0;
+    }
   }
   s.own_len = 0;
   s.before = 0;
 #pragma unroll
   for (int i = 0; i < kKv8MaxSeg; ++i) {
-    s.len[i] = max(s.len[i], 0);
     if (i == s.nseg - 1) s.own_len = s.len[i];
     if (i < s.nseg - 1) s.before += s.len[i];
   }

@@ -76,3 +76,45 @@ def test_a_block_before_its_sequence_is_reported(QH, KH, D):
     blocks[0, 1] = -64
     ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1, out=out)
     assert ops.read_and_clear_error(0) == 5 and bool((out == 7).all())
+
+
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+@pytest.mark.parametrize("length,off", [(33, 0), (2 ** 31 - 1, 0), (2 ** 31 - 1, 1), (17, 1), (1, 2), (20, -1),
+                                        (1, -2 ** 31), (20, 2 ** 31 - 1)])
+def test_a_segment_past_the_page_list_is_reported_and_empty(QH, KH, D, length, off):
+    # its keys would be looked up outside the list, and lengths like these pass 32 bits when summed
+    q, kp, vp, seqs, blocks, pl = one_sequence(QH, KH, D)
+    for p in (kp, vp):
+        p.codes.random_(-127, 128)
+        p.bytes.fill_(120)
+    seqs[0, 2], seqs[0, 4], seqs[0, 8], seqs[0, 5], seqs[0, 9] = 2, length, off, 20, 0
+    alone = seqs.clone()
+    alone[0, 2], alone[0, 4], alone[0, 8] = 1, 20, 0
+    n = 40
+    many = seqs.expand(n, -1).contiguous()
+    dseqs = torch.arange(n, **I32)
+    got = ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1)
+    assert ops.read_and_clear_error(0) == 5
+    want = ops.prefill_attention_kv8(q, kp, vp, alone, blocks, pl, 0.1)
+    assert ops.read_and_clear_error(0) == 0 and torch.equal(got, want)
+    got = torch.zeros_like(want)
+    ops.decode_attention_kv8(q, kp, vp, many, dseqs, pl, 0.1, out=got)
+    assert ops.read_and_clear_error(0) == 5
+    want = torch.zeros_like(want)
+    ops.decode_attention_kv8(q, kp, vp, alone.expand(n, -1).contiguous(), dseqs, pl, 0.1, out=want)
+    assert ops.read_and_clear_error(0) == 0 and torch.equal(got, want)
+
+
+def test_a_page_list_past_32_bit_sums_is_refused():
+    q, kp, vp, seqs, blocks, pl = one_sequence(8, 2, 128)
+    pl = torch.zeros(2 ** 25 + 1, **I32)
+    with pytest.raises(RuntimeError, match="page list"):
+        ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1)
+    with pytest.raises(RuntimeError, match="page list"):
+        ops.decode_attention_kv8(q, kp, vp, seqs, torch.zeros(1, **I32), pl, 0.1)
+    # the largest one allowed: a launch takes as many rows as 32-bit counts of its tiles allow
+    pl = torch.zeros(2 ** 25 - 1, **I32)
+    n = 100
+    out = torch.zeros(q.shape[0], 8 * 128, dtype=torch.bfloat16, device=DEV)
+    ops.decode_attention_kv8(q, kp, vp, seqs.expand(n, -1).contiguous(), torch.arange(n, **I32), pl, 0.1, out=out)
+    ops.prefill_attention_kv8(q, kp, vp, seqs, blocks, pl, 0.1)
