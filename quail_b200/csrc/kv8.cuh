@@ -24,6 +24,7 @@ namespace qb {
 
 constexpr int kKv8Block = 16;        // tokens per exponent byte
 constexpr int kKv8MinByte = 67;
+constexpr int kKv8TopByte = 248;       // of int8; e4m3 needs no more than 247
 constexpr int kKv8Nan = 255;
 constexpr int kKv8SeqInts = 12;
 constexpr int kKv8MaxSeg = 4;
@@ -31,14 +32,21 @@ constexpr int kKv8MaxSeg = 4;
 // Exponent byte for a block whose largest magnitude has these fp32 bits: the
 // smallest power of two with 127 * 2^e (int8) or 448 * 2^e (e4m3) >= amax.
 // 127 = 1.984375 * 2^6 and 448 = 1.75 * 2^8, so a compare of the mantissa decides.
+// int8's 249 is not used: its codes from 64 on would stand for 2^128 and more, past fp32 and bf16 (kv8_top).
 template <bool FP8>
 __device__ __forceinline__ int kv8_byte(uint32_t amax_bits) {
   if (amax_bits >= 0x7f800000u) return kKv8Nan;
   const int x = (int)(amax_bits >> 23);
   const uint32_t frac = amax_bits & 0x7fffffu;
-  const int b = FP8 ? x - 8 + (frac > 0x600000u) : x - 6 + (frac > 0x7e0000u);
+  const int b = FP8 ? x - 8 + (frac > 0x600000u) : min(x - 6 + (frac > 0x7e0000u), kKv8TopByte);
   return max(b, kKv8MinByte);
 }
+
+// The largest magnitude that is stored; finite values above it become it. int8: 127 * 2^(248 - 127), within half a
+// step of bf16's largest number. e4m3's 4 bits would round a magnitude from 1.9375 * 2^127 up to 2^128, which no
+// reader's bf16 holds: 1.875 * 2^127 is the largest code below it.
+template <bool FP8>
+constexpr float kv8_top = FP8 ? 3.1901471898837980e38f : 3.3762391092936860e38f;
 
 // 2^(byte - 127) as fp32; NaN for 255
 __device__ __forceinline__ float kv8_scale(int byte) {

@@ -77,10 +77,6 @@ __device__ __forceinline__ uint8_t encode(float y) {
   }
 }
 
-// e4m3's 4 bits would round a magnitude from 1.9375 * 2^127 up to 2^128, which no reader's bf16
-// holds: such values become the largest code below it
-constexpr float kTopE4m3 = 3.1901471898837980e38f;   // 1.875 * 2^127
-
 template <bool FP8>
 __device__ __forceinline__ float decode(uint8_t c) {
   if constexpr (FP8) {
@@ -224,7 +220,7 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(const __grid_constant__ 
       __align__(8) uint8_t y[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        if (FP8) v[i] = fminf(fmaxf(v[i], -kTopE4m3), kTopE4m3);
+        v[i] = fminf(fmaxf(v[i], -kv8_top<FP8>), kv8_top<FP8>);
         y[i] = byte == kKv8Nan ? 0 : encode<FP8>(v[i] * inv);
       }
       store_codes<N>(codes + (size_t)o * D, y);

@@ -119,24 +119,26 @@ def segmented_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     return out
 
 
-KV8_MIN_BYTE, KV8_NAN_BYTE = 67, 255
+KV8_MIN_BYTE, KV8_INT8_TOP_BYTE, KV8_NAN_BYTE = 67, 248, 255
 
 
 def kv8_byte(amax: torch.Tensor, dtype) -> torch.Tensor:
     """Exponent byte of blocks whose largest magnitude is amax: the smallest power of two times the
-    largest code (127, or 448 of e4m3) that reaches it, at least 2^-60; 255 when amax is not finite."""
+    largest code (127, or 448 of e4m3) that reaches it, at least 2^-60 and, for int8, at most 2^121 (whose largest
+    code is the largest value stored); 255 when amax is not finite."""
     m, e = torch.frexp(amax.double())
     top, shift = (127 / 128, 7) if dtype == torch.int8 else (448 / 512, 9)
     b = e - shift + (m > top).to(e.dtype) + 127
-    b = torch.where(amax > 0, b, torch.zeros_like(b)).clamp(min=KV8_MIN_BYTE)
+    b = torch.where(amax > 0, b, torch.zeros_like(b)).clamp(KV8_MIN_BYTE,
+                                                            KV8_INT8_TOP_BYTE if dtype == torch.int8 else None)
     return torch.where(torch.isfinite(amax), b, torch.full_like(b, KV8_NAN_BYTE)).to(torch.int64)
 
 
 def kv8_encode(x: torch.Tensor, byte: torch.Tensor, dtype) -> torch.Tensor:
     """Codes of values x under exponent bytes (broadcast): round(x * 2^(127 - byte)), nearest even."""
     x = x.double()
-    if dtype != torch.int8:
-        x = x.clamp(-1.875 * 2.0 ** 127, 1.875 * 2.0 ** 127)          # not to 2^128, past bf16's range
+    top = (127 / 64 if dtype == torch.int8 else 1.875) * 2.0 ** 127   # not to 2^128, past bf16's range
+    x = x.clamp(-top, top)
     y = x * torch.exp2(127.0 - byte.double())
     y = torch.where(byte == KV8_NAN_BYTE, torch.zeros_like(y), y)
     return torch.round(y).to(torch.int8) if dtype == torch.int8 else y.float().to(dtype)

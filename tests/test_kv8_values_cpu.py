@@ -1,0 +1,23 @@
+"""The 8-bit KV cache's statements at the ends of their range."""
+
+import pytest
+import torch
+
+from quail_b200.ops import KV8_DTYPES, Pages8
+from quail_b200.ops import reference as ref
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_every_finite_value_is_stored_as_a_bf16_number(kind):
+    dtype = KV8_DTYPES[kind]
+    x = torch.tensor([torch.finfo(torch.float32).max, torch.finfo(torch.bfloat16).max, 2.0 ** 127 * 127 / 64,
+                      2.0 ** 127 * 1.875, 2.0 ** 127, 3.3e38, 1.0, 0.0])
+    p = Pages8.zeros(1, 16, 1, 64, dtype, "cpu")
+    rows = torch.zeros(8, 1, 64)
+    rows[:, 0, 0], rows[:, 0, 1] = x, -x
+    ref.kv8_write(rows, torch.arange(8, dtype=torch.int32), p.codes, p.bytes)
+    got = ref.kv8_values(p.codes, p.bytes)[0, :8, 0]
+    assert bool((got.abs() < 2.0 ** 128).all()) and torch.equal(got, got.float().bfloat16().double())
+    assert torch.equal(got[:, 0], -got[:, 1])
+    top = 2.0 ** 127 * (127 / 64 if kind == "int8" else 1.875)
+    assert got[0, 0] == got[1, 0] == top and got[4, 0] == 2.0 ** 127

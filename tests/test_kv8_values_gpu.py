@@ -1,0 +1,41 @@
+"""8-bit KV operators on values, scales and masks at the ends of their ranges, against the 64-bit statements
+(bounds as in test_kv8_gpu.py)."""
+
+
+import pytest
+import torch
+
+from quail_b200 import ops
+from test_kv8_gpu import DEV, KINDS, write_both
+
+pytestmark = pytest.mark.gpu
+
+TOP = {d: torch.finfo(d).max for d in (torch.bfloat16, torch.float32)}
+
+
+@pytest.fixture(autouse=True)
+def _no_kernel_errors():
+    torch.manual_seed(0)
+    yield
+    assert ops.read_and_clear_error(0) == 0
+
+
+# ------------------------------------------------------------------ write and read
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_largest_finite_values_stay_finite(kind, dtype):
+    P, KH, D = 16, 2, 128
+    kp, vp = (ops.Pages8.zeros(3, P, KH, D, ops.KV8_DTYPES[kind], DEV) for _ in range(2))
+    rows = torch.randn(32, KH, D, device=DEV).to(dtype)
+    rows[3, 0, 5], rows[4, 0, 6], rows[20, 1, 0] = TOP[dtype], -TOP[dtype], 3.38e38
+    rows[5, 0] = 0
+    slots = torch.arange(32, dtype=torch.int32, device=DEV)
+    write_both(rows, -rows, slots, kp, vp)
+    k, v = ops.kv8_read(kp, vp, slots)
+    assert bool(torch.isfinite(k).all()) and bool(torch.isfinite(v).all()) and not bool(k[5, 0].any())
+    # int8: half a step of 2^(byte - 127), a whole one for fp32 values past 127.5 of them; e4m3: 4 significant bits
+    # and steps of 2^-9, and its largest value below 2^128 is 1.875 * 2^127
+    step = torch.exp2(kp.bytes[:2].double() - 127).permute(0, 2, 1).repeat_interleave(16, dim=1).reshape(32, KH, 1)
+    x = rows.double()
+    bound = (0.5 if dtype == torch.bfloat16 else 1.0) * step if kind == "int8" else x.abs() * 2 ** -4 + step * 2 ** -10
+    assert bool(((k.double() - x).abs() <= bound).all()) and bool(((v.double() + x).abs() <= bound).all())
