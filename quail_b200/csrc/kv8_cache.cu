@@ -6,7 +6,7 @@
 // (but for fewer than 16 skipped rows among them).
 // One warp owns a run of K or of V of one head: it takes the largest magnitude
 // (an integer max over |x| bits), grows the block's byte if it has to, rescales
-// the older codes of the block when the byte grew, and writes the new codes.
+// the block's other codes when the byte grew, and writes the new codes.
 // No two warps touch one block, so there are no atomics and the result does not
 // depend on timing. Bound by the bytes: each row is read (bf16) and half as
 // many bytes are written.
@@ -115,8 +115,10 @@ struct WriteArgs {
 
 // GROUP tokens per warp: 1 (few rows: every row's own warp) or 16 (a packed
 // chunk: at most two runs begin in 16 adjacent rows of one sequence).
+// Four CTAs an SM are kept up to head_dim 128 (the compiler's own 136 registers leave three: write and read of 16k
+// tokens 81 us, with four 73); at 256 the rows held would spill.
 template <typename T, int D, bool FP8, bool VEC, int GROUP>
-__global__ void __launch_bounds__(128) kv8_write_kernel(const __grid_constant__ WriteArgs a) {
+__global__ void __launch_bounds__(128, D == 256 ? 1 : 4) kv8_write_kernel(const __grid_constant__ WriteArgs a) {
   constexpr int N = D / 32;
   const int lane = threadIdx.x & 31;
   const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
@@ -166,7 +168,7 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(const __grid_constant__ 
     const int s1 = __shfl_sync(0xffffffffu, slot2, (l0 + lane) & 31);
     const int off = (l0 + lane < 32 ? s0 : s1) & (kKv8Block - 1);      // of row t0 + l0 + lane
     const uint32_t fresh = __reduce_or_sync(0xffffffffu, (run >> lane) & 1 ? 1u << off : 0u);
-    const int first = __ffs(fresh) - 1, last = 31 - __clz(fresh);
+    const int first = __ffs(fresh) - 1;
     // a run without skipped rows of at most 256 bytes a row is read once, all 16 rows in flight
     constexpr bool kHold = VEC && N * sizeof(T) <= 16;
     const bool held = kHold && run == (0xffffffffu >> (32 - span)) && span <= kKv8Block;
@@ -200,11 +202,11 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(const __grid_constant__ 
       const int old = *byte_p;
       byte = max(byte, old);
       if (byte != old) {
-        // the block's scale grew: its older rows move to the new one, rounded once
+        // the block's scale grew: all its other rows, those after the new ones too, move to the new one, rounded once
         const int d = old - byte;
         const float f = d < -126 ? 0.f : __uint_as_float((uint32_t)(127 + d) << 23);
 #pragma unroll 4
-        for (int r = 0; r < last; ++r) {
+        for (int r = 0; r < kKv8Block; ++r) {
           if ((fresh >> r) & 1) continue;
           Codes<N> c;
           __align__(8) uint8_t y[N];

@@ -83,9 +83,9 @@ def kv8_write(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_pages: Pa
 
     slots int32 [T]: page * P + offset, -1 to skip a row. The rows of one 16-token block are
     adjacent in the call (a sequence's new tokens in order are), with fewer than 16 skipped
-    rows between them. A block's exponent grows to
-    what its largest value needs, and the codes it already holds are rescaled (rounded once);
-    a write at a block's offset 0 begins it anew. A value that is not finite marks its block:
+    rows between them. A block's exponent grows to what its largest value needs, and the
+    codes of all its other rows are rescaled (rounded once); a write at a block's offset 0
+    begins it anew, and its other rows are lost. A value that is not finite marks its block:
     attention over it gives NaN.
     """
     K.count_launch()

@@ -171,7 +171,7 @@ def kv8_write(x: torch.Tensor, slots: torch.Tensor, codes: torch.Tensor, byte: t
         if min(offs) > 0:
             old = byte[page, :, at].long()
             b = torch.maximum(b, old)
-            for o in range(max(offs)):
+            for o in range(16):
                 if o not in offs:
                     c = codes[page, :, at * 16 + o].double()
                     raw[page, :, at * 16 + o] = kv8_encode(c * torch.exp2(old.double() - 127)[:, None], b[:, None],

@@ -21,3 +21,13 @@ def test_every_finite_value_is_stored_as_a_bf16_number(kind):
     assert torch.equal(got[:, 0], -got[:, 1])
     top = 2.0 ** 127 * (127 / 64 if kind == "int8" else 1.875)
     assert got[0, 0] == got[1, 0] == top and got[4, 0] == 2.0 ** 127
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_a_row_written_before_kept_rows_of_its_block_leaves_their_values(kind):
+    p = Pages8.zeros(1, 16, 2, 64, KV8_DTYPES[kind], "cpu")
+    ref.kv8_write(torch.ones(16, 2, 64), torch.arange(16, dtype=torch.int32), p.codes, p.bytes)
+    ref.kv8_write(torch.full((1, 2, 64), 8.0), torch.tensor([3], dtype=torch.int32), p.codes, p.bytes)
+    want = torch.ones(16, 2, 64, dtype=torch.float64)
+    want[3] = 8
+    assert torch.equal(ref.kv8_values(p.codes, p.bytes)[0], want)

@@ -1,7 +1,6 @@
 """8-bit KV operators on values, scales and masks at the ends of their ranges, against the 64-bit statements
 (bounds as in test_kv8_gpu.py)."""
 
-
 import pytest
 import torch
 
@@ -39,3 +38,20 @@ def test_the_largest_finite_values_stay_finite(kind, dtype):
     x = rows.double()
     bound = (0.5 if dtype == torch.bfloat16 else 1.0) * step if kind == "int8" else x.abs() * 2 ** -4 + step * 2 ** -10
     assert bool(((k.double() - x).abs() <= bound).all()) and bool(((v.double() + x).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_row_written_before_kept_rows_of_its_block_leaves_their_values(kind):
+    P, KH, D = 16, 2, 128
+    for first in (1, 3, 14):
+        kp, vp = (ops.Pages8.zeros(3, P, KH, D, ops.KV8_DTYPES[kind], DEV) for _ in range(2))
+        ones = torch.ones(16, KH, D, device=DEV).bfloat16()
+        write_both(ones, ones, torch.arange(16, 32, dtype=torch.int32, device=DEV), kp, vp)
+        big = 8 * ones[:1]
+        write_both(big, -big, torch.tensor([16 + first], dtype=torch.int32, device=DEV), kp, vp)
+        k, v = ops.kv8_read(kp, vp, torch.arange(16, 32, dtype=torch.int32, device=DEV))
+        want = torch.ones(16, KH, D, device=DEV).bfloat16()
+        want[first] = 8
+        assert torch.equal(k, want)
+        want[first] = -8
+        assert torch.equal(v, want)
