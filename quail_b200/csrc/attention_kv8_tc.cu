@@ -548,9 +548,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (ct < 4) {
-          const int kb = (raw_info[8 * rs] >> (8 * ct)) & 0xff, vb = (raw_info[8 * rs + 1] >> (8 * ct)) & 0xff;
+          const int kb = (raw_info[8 * rs] >> (8 * ct)) & 0xff;
+          // a block never written has a byte of 0 and codes of 0: no byte below the smallest that is written,
+          // as p 2^(byte - 127) would underflow and the block's share of the sum with it
+          const int vb = max((raw_info[8 * rs + 1] >> (8 * ct)) & 0xff, kKv8MinByte);
           float* sc = scales + st * kScaleFloats;
-          sc[ct] = kv8_scale(kb) * (a.sl2 / kv8_unit<FP8>);
+          // never 0 (a softmax scale of 0, a byte of 0): a masked score is -inf, and has to stay that
+          sc[ct] = kb == kKv8Nan ? kv8_scale(kb) : fmaxf(kv8_scale(kb) * (a.sl2 / kv8_unit<FP8>), 1.1754943508222875e-38f);
           // p is stored times 2^(vb - 127) / unit
           const float shift = (float)(vb - 127) - (FP8 ? 0.f : -6.f);
           sc[4 + ct] = vb == kKv8Nan ? __int_as_float(0x7fc00000) : shift;

@@ -1,14 +1,16 @@
 """8-bit KV operators on values, scales and masks at the ends of their ranges, against the 64-bit statements
 (bounds as in test_kv8_gpu.py)."""
 
+
 import pytest
 import torch
 
 from quail_b200 import ops
-from test_kv8_gpu import DEV, KINDS, write_both
+from test_kv8_gpu import DEV, KINDS, blocks_of, check_rows, layout, random_pages, write_both
 
 pytestmark = pytest.mark.gpu
 
+GEOMETRIES = [(8, 2, 128), (16, 2, 128), (4, 2, 128), (4, 1, 256), (4, 4, 64)]      # tcgen05 and mma.sync prefill
 TOP = {d: torch.finfo(d).max for d in (torch.bfloat16, torch.float32)}
 
 
@@ -55,3 +57,45 @@ def test_a_row_written_before_kept_rows_of_its_block_leaves_their_values(kind):
         assert torch.equal(k, want)
         want[first] = -8
         assert torch.equal(v, want)
+
+
+# ------------------------------------------------------------------ attention
+def both(q, kp, vp, seqs, pl, scale):
+    """Prefill and decode against the statement; decode once as few short rows and once over a long page list."""
+    lse = torch.empty(q.shape[0], q.shape[1], device=DEV)
+    out = ops.prefill_attention_kv8(q, kp, vp, seqs, blocks_of(seqs), pl, scale, lse=lse)
+    check_rows(out, lse, q, kp, vp, seqs, pl, scale)
+    dseqs = torch.arange(seqs.shape[0], dtype=torch.int32, device=DEV)
+    last = (seqs[:, 0] + seqs[:, 1] - 1).long()
+    for table in (pl, torch.cat([pl, pl.new_zeros(8192)])):
+        dec = torch.zeros_like(out)
+        ops.decode_attention_kv8(q, kp, vp, seqs, dseqs, table, scale, out=dec, lse=lse)
+        check_rows(dec, lse, q, kp, vp, seqs, pl, scale, last)
+    return out
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+def test_attention_over_blocks_never_written(kind, QH, KH, D):
+    # zeros with an exponent byte of 0: keys and values of 0, in and beyond a causal mask's edge
+    P, pages = 64, 16
+    kp, vp = random_pages(pages, KH, P, D, kind, 41), random_pages(pages, KH, P, D, kind, 42)
+    seqs, pl, T = layout([(100, [30, 100]), (20, [90, 20]), (1, [70])], P, pages)
+    q = torch.randn(T, QH, D, device=DEV).bfloat16()
+    for blank in ([0, 1, 2, 3], [1]):
+        for p in (kp, vp):
+            for e in pl.tolist():
+                p.codes[e, :, :].view(torch.uint8).view(KH, P // 16, 16, D)[:, blank] = 0
+                p.bytes[e][:, blank] = 0
+        both(q, kp, vp, seqs, pl, 0.1)
+        kp, vp = random_pages(pages, KH, P, D, kind, 43), random_pages(pages, KH, P, D, kind, 44)
+
+
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+def test_a_softmax_scale_of_zero_is_the_mean(QH, KH, D):
+    P, pages = 64, 12
+    kp, vp = random_pages(pages, KH, P, D, "int8", 45), random_pages(pages, KH, P, D, "int8", 46)
+    seqs, pl, T = layout([(100, [30, 100]), (1, [70])], P, pages)
+    q = torch.randn(T, QH, D, device=DEV).bfloat16()
+    both(q, kp, vp, seqs, pl, 0.0)
+    both(q, kp, vp, seqs, pl, 1e-30)
