@@ -18,6 +18,8 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 
+#include <cmath>
+
 #include "kv8.cuh"
 #include "mx_common.cuh"
 
@@ -371,6 +373,9 @@ Kv8Attn kv8_args(const char* what, const torch::Tensor& q, const torch::Tensor& 
   TORCH_CHECK(out.dim() == 2 && out.size(0) == T && out.size(1) == QH * D && out.is_contiguous() &&
                   out.device() == q.device(),
               what, ": out [T, QH*D]");
+  // a row's largest score is found before the scale is applied
+  TORCH_CHECK(scale >= 0 && std::isfinite((float)(scale * 1.4426950408889634)), what,
+              ": the softmax scale is finite and not negative");
   // the kernels sum a sequence's (at most 4) segments, none longer than the list, in 32 bits
   TORCH_CHECK(page_list.numel() <= INT32_MAX / kKv8MaxSeg / kc.size(2), what, ": the page list passes 2^29 tokens");
   Kv8Attn a;

@@ -121,7 +121,7 @@ def prefill_attention_kv8(q, k_pages: Pages8, v_pages: Pages8, seqs, blocks, pag
     blocks [m, 2] int32: (sequence, first query token) per 64-token block (a chunk's `blocks`);
     rows no block covers are not written. Returns bf16, or with fp8_out (e4m3, UE8M0 scale bytes
     in the MX atom layout). A row that sees no key is 0 (and -inf in `lse`, fp32 [T, QH], which
-    goes with a bf16 output).
+    goes with a bf16 output). softmax_scale is finite and at least 0.
     """
     _check_heads("prefill_attention_kv8", q, k_pages)
     out, out_scale = _outputs(q, fp8_out, out, out_scale)

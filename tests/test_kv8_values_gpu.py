@@ -99,3 +99,15 @@ def test_a_softmax_scale_of_zero_is_the_mean(QH, KH, D):
     q = torch.randn(T, QH, D, device=DEV).bfloat16()
     both(q, kp, vp, seqs, pl, 0.0)
     both(q, kp, vp, seqs, pl, 1e-30)
+
+
+def test_a_softmax_scale_that_is_negative_or_not_finite_is_refused():
+    P, pages, QH, KH, D = 64, 12, 8, 2, 128
+    kp, vp = random_pages(pages, KH, P, D, "int8", 45), random_pages(pages, KH, P, D, "int8", 46)
+    seqs, pl, T = layout([(100, [30, 100]), (1, [70])], P, pages)
+    q = torch.randn(T, QH, D, device=DEV).bfloat16()
+    for scale in (-0.1, float("nan"), float("inf"), 1e39):
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.prefill_attention_kv8(q, kp, vp, seqs, blocks_of(seqs), pl, scale)
+        with pytest.raises(RuntimeError, match="scale"):
+            ops.decode_attention_kv8(q, kp, vp, seqs, torch.zeros(1, dtype=torch.int32, device=DEV), pl, scale)
