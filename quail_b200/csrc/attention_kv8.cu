@@ -199,7 +199,8 @@ __global__ void __launch_bounds__(128) attn_kv8_kernel(const __grid_constant__ K
                            kv8_hi<FP8>(wv[2 * u + 1]));
       }
     }
-    if (tid < 2 * (BK / 16)) sScale[tid] = kv8_scale(rbyte) / kv8_unit<FP8>;
+    if (tid < 2 * (BK / 16))
+      sScale[tid] = kv8_scale(rbyte) * ((tid < BK / 16 ? 1.f : kKv8Down) / kv8_unit<FP8>);
     __syncthreads();
     more = advance();
     if (more) fetch();
@@ -284,7 +285,7 @@ __global__ void __launch_bounds__(128) attn_kv8_kernel(const __grid_constant__ K
     float l = l_run[r];
     l += __shfl_xor_sync(0xffffffffu, l, 1);
     l += __shfl_xor_sync(0xffffffffu, l, 2);
-    const float inv = l == 0.f ? 0.f : 1.f / l;      // no visible key: 0; NaN stays NaN
+    const float inv = l == 0.f ? 0.f : kKv8Up / l;   // no visible key: 0; NaN stays NaN
     const size_t row = (size_t)tok[r] * a.QH + head[r];
     if constexpr (!MX) {
       if (valid[r]) {
@@ -303,13 +304,14 @@ __global__ void __launch_bounds__(128) attn_kv8_kernel(const __grid_constant__ K
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const uint8_t e = ue8m0_of(amax);
-        const float f = ue8m0_inv(e) * inv;
+        const float f = ue8m0_inv(e);                // not times inv, which may pass fp32
         if (valid[r]) {
           uint8_t* dst = a.o8 + row * D + c * 32 + t4 * 2;
 #pragma unroll
           for (int d = 0; d < 4; ++d)
             *reinterpret_cast<__nv_fp8x2_storage_t*>(dst + d * 8) = __nv_cvt_float2_to_fp8x2(
-                make_float2(oacc[4 * c + d][2 * r] * f, oacc[4 * c + d][2 * r + 1] * f), __NV_SATFINITE, __NV_E4M3);
+                make_float2(oacc[4 * c + d][2 * r] * inv * f, oacc[4 * c + d][2 * r + 1] * inv * f), __NV_SATFINITE,
+                __NV_E4M3);
           if (t4 == 0) {
             const int col = head[r] * D + c * 32, t = tok[r];
             a.osf[((size_t)(t >> 7) * (a.QH * D / 128) + col / 128) * 512 + (t & 31) * 16 + ((t & 127) >> 5) * 4 +

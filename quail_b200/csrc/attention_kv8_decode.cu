@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(DecGeom<D>::kWarps * 32, DecGeom<D>::kBlocksPe
       const bool full = lo == 0 && hi == kTile;
       const uint8_t* sk = smem + (warp * NS + st) * Gm::kStageBytes;
       const uint8_t* sv = sk + Gm::kSide;
-      const float mine_scale = kv8_scale(ti.byte) * (lane & 2 ? 1.f / kv8_unit<FP8> : 1.f);
+      const float mine_scale = kv8_scale(ti.byte) * (lane & 2 ? kKv8Down / kv8_unit<FP8> : 1.f);
       // row g of a block's product is key kg of the block, row g + 8 key kg + 2
       const int kg = (g >> 1) * 4 + (g & 1);
       float s[2][4];
@@ -675,7 +675,7 @@ __global__ void __launch_bounds__(DecGeom<D>::kWarps * 32, DecGeom<D>::kBlocksPe
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         const int hl = 2 * t4 + hh;
-        const float inv = !whole ? 1.f : ls[hh] == 0.f ? 0.f : 1.f / ls[hh];
+        const float inv = !whole ? 1.f : ls[hh] == 0.f ? 0.f : kKv8Up / ls[hh];
 #pragma unroll
         for (int u = 0; u < (D == 256 ? 2 : 1); ++u) {
           float v[C];
@@ -744,7 +744,7 @@ __global__ void __launch_bounds__(DecGeom<D>::kWarps * 32, DecGeom<D>::kBlocksPe
 #pragma unroll
         for (int k = 0; k < N; ++k) v[k] += part(w)[hl * D + lane * N + k] * c;
       }
-      const float inv = l_ == 0.f ? 0.f : 1.f / l_;
+      const float inv = l_ == 0.f ? 0.f : kKv8Up / l_;
 #pragma unroll
       for (int k = 0; k < N; ++k) v[k] *= inv;
       if (p_row < 0) break;                                                // alike in the CTA
@@ -850,7 +850,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   }
   const int row = c.row;
   if (row < 0) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : kKv8Up / l;
 #pragma unroll
   for (int k = 0; k < N; ++k) v[k] *= inv;
   const int head = (c.hg / HG) * G + (c.hg % HG) * kHeads + hl;

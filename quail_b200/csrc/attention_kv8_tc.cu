@@ -60,7 +60,7 @@ constexpr int kQBytes = kRows * 256;           // a tile: two 64-dim atoms of 12
 constexpr int kTileBytes = kKeys * 256;        // K or V as bf16: two atoms of 64 rows
 constexpr int kRawBytes = 2 * kKeys * kD;      // codes of K, then of V
 constexpr int kPBytes = kRows * 128;
-constexpr int kScaleFloats = 16;               // per stage: K units [4], V log2 [4], V inverses [4], masks [3]
+constexpr int kScaleFloats = 20;               // per stage: K units [4], V log2 [4], V inverses [4], masks [3], tops [4]
 constexpr int kItems = 4;                     // item descriptors in flight
 constexpr int kBarBytes = 1024;
 constexpr int kSmem = 2 * kQBytes + kStages * 2 * kTileBytes + kRaw * kRawBytes + 2 * kPBytes + kBarBytes + 1024;
@@ -143,6 +143,11 @@ __device__ __forceinline__ uint32_t pack_bf2(float lo, float hi) {
   return r;
 }
 
+// p reaches 2^8 (the running maximum may be that far behind), a code 2 (int8) or 2^9 (e4m3), and 2^24 keys may add up
+// below 2^128: where the V exponent is above this, the running maximum is taken that much higher.
+template <bool FP8>
+constexpr int kTopShift = FP8 ? 84 : 92;
+
 // A work item's geometry, as the loader hands it to the other roles.
 struct Item {
   int tok, head0;              // first query row and head
@@ -181,7 +186,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* item_empty = item_full + kItems;            // [kItems] count 14: every warp but the loader
   int* raw_info = reinterpret_cast<int*>(bars + 32);    // [kRaw][8]: 4 bytes of K, 4 of V, and the masks' numbers
   float* scales = reinterpret_cast<float*>(bars + 40);  // [kStages][kScaleFloats]
-  Item* items = reinterpret_cast<Item*>(bars + 64);     // [kItems]
+  Item* items = reinterpret_cast<Item*>(bars + 72);     // [kItems]
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int groups = a.QH / 4;
@@ -556,9 +561,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           // never 0 (a softmax scale of 0, a byte of 0): a masked score is -inf, and has to stay that
           sc[ct] = kb == kKv8Nan ? kv8_scale(kb) : fmaxf(kv8_scale(kb) * (a.sl2 / kv8_unit<FP8>), 1.1754943508222875e-38f);
           // p is stored times 2^(vb - 127) / unit
-          const float shift = (float)(vb - 127) - (FP8 ? 0.f : -6.f);
-          sc[4 + ct] = vb == kKv8Nan ? __int_as_float(0x7fc00000) : shift;
-          sc[8 + ct] = vb == kKv8Nan ? __int_as_float(0x7fc00000) : kv8_ex2(-shift);
+          const int shift = vb - 127 + (FP8 ? 0 : 6);
+          sc[4 + ct] = vb == kKv8Nan ? __int_as_float(0x7fc00000) : (float)shift;
+          sc[8 + ct] = vb == kKv8Nan ? __int_as_float(0x7fc00000) : scalbnf(1.f, -shift);   // 2^-127 too
+          sc[16 + ct] = (float)max(shift - kTopShift<FP8>, 0);
           if (ct < 3) sc[12 + ct] = __int_as_float(raw_info[8 * rs + 2 + ct]);
         }
         fence_proxy_async_smem();
@@ -618,6 +624,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float4 vi = *reinterpret_cast<const float4*>(scales + st * kScaleFloats + 8);
         const float kfs[4] = {kf.x, kf.y, kf.z, kf.w}, vfs[4] = {vf.x, vf.y, vf.z, vf.w};
         const float vis[4] = {vi.x, vi.y, vi.z, vi.w};
+        const float4 vt = *reinterpret_cast<const float4*>(scales + st * kScaleFloats + 16);
+        const float vts[4] = {vt.x, vt.y, vt.z, vt.w};
         const int4 mk = *reinterpret_cast<const int4*>(scales + st * kScaleFloats + 12);
         const int lo = pos + mk.z, hi = valid ? min(mk.x, pos + mk.y) : 0;
         const bool full = __all_sync(0xffffffffu, lo <= 0 && hi >= kKeys);
@@ -636,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 5; ++i)
             y[i] = max3(__uint_as_float(x[3 * i]), __uint_as_float(x[3 * i + 1]), __uint_as_float(x[3 * i + 2]));
           const float z = max3(max3(y[0], y[1], y[2]), max3(y[3], y[4], __uint_as_float(x[15])), -INFINITY);
-          tmax = fmaxf(tmax, z * kfs[b]);
+          tmax = fmaxf(tmax, fmaf(z, kfs[b], vts[b]));
         }
         float corr = 1.f;
         if (tmax > m_ref + 8.f) {

@@ -102,6 +102,10 @@ __device__ __forceinline__ uint32_t kv8_half2(uint32_t x) {
   return r;
 }
 
+// A mean of values near fp32's largest is finite, their sum is not: the mma.sync kernels take V's scales times 2^-24
+// and their results times 2^24, which is room for 2^24 keys. (The tcgen05 kernel raises its running maximum instead.)
+constexpr float kKv8Down = 5.9604644775390625e-8f, kKv8Up = 16777216.f;
+
 __device__ __forceinline__ float kv8_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -1,6 +1,7 @@
 """8-bit KV operators on values, scales and masks at the ends of their ranges, against the 64-bit statements
 (bounds as in test_kv8_gpu.py)."""
 
+import math
 
 import pytest
 import torch
@@ -72,6 +73,32 @@ def both(q, kp, vp, seqs, pl, scale):
         ops.decode_attention_kv8(q, kp, vp, seqs, dseqs, table, scale, out=dec, lse=lse)
         check_rows(dec, lse, q, kp, vp, seqs, pl, scale, last)
     return out
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+@pytest.mark.parametrize("top", [2.0 ** 100, 2.0 ** 122, 3.38e38])
+def test_attention_over_large_values(kind, QH, KH, D, top):
+    # the mean of values near the largest number is finite, though their sum is not, nor p 2^8 times one of them
+    # (a running maximum may be that far behind)
+    P, pages = 64, 16
+    kp, vp = (ops.Pages8.zeros(pages, P, KH, D, ops.KV8_DTYPES[kind], DEV) for _ in range(2))
+    seqs, pl, T = layout([(70, [200, 70]), (3, [130]), (1, [1])], P, pages)
+    n = 200 + 70 + 130 + 1
+    g = torch.arange(n, device=DEV).view(-1, 1, 1) % 200
+    k = (0.3 + 0.004 * g + 0.01 * torch.rand(n, KH, D, device=DEV)).bfloat16()          # scores grow slowly
+    v = (top * (0.6 + 0.4 * torch.rand(n, KH, D, device=DEV))).clamp(max=TOP[torch.bfloat16]).bfloat16()
+    v[::7] = -v[::7]
+    v[1::2] *= 2.0 ** -30
+    order = []
+    for row in seqs.tolist():
+        for i in range(row[2]):
+            order += [int(pl[row[8 + i] + j // P]) * P + j % P for j in range(row[4 + i])]
+    slots = torch.tensor(order, dtype=torch.int32, device=DEV)
+    ops.kv8_write(k, v, slots, kp, vp)
+    q = (0.5 + torch.rand(T, QH, D, device=DEV)).bfloat16()
+    out = both(q, kp, vp, seqs, pl, 1 / math.sqrt(D))
+    assert bool(torch.isfinite(out).all())
 
 
 @pytest.mark.parametrize("kind", KINDS)
