@@ -627,7 +627,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float4 vt = *reinterpret_cast<const float4*>(scales + st * kScaleFloats + 16);
         const float vts[4] = {vt.x, vt.y, vt.z, vt.w};
         const int4 mk = *reinterpret_cast<const int4*>(scales + st * kScaleFloats + 12);
-        const int lo = pos + mk.z, hi = valid ? min(mk.x, pos + mk.y) : 0;
+        const int lo = pos + mk.z, end = valid ? min(mk.x, pos + mk.y) : 0;
+        const int hi = end > lo ? end : 0;              // a window may end before its tile's first key, or after its last
         const bool full = __all_sync(0xffffffffu, lo <= 0 && hi >= kKeys);
         tmem_ld_wait();
         if (!full) {

@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from quail_b200 import ops
+from quail_b200.ops import reference as ref
 from test_kv8_gpu import DEV, KINDS, blocks_of, check_rows, layout, random_pages, write_both
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +139,19 @@ def test_a_softmax_scale_that_is_negative_or_not_finite_is_refused():
             ops.prefill_attention_kv8(q, kp, vp, seqs, blocks_of(seqs), pl, scale)
         with pytest.raises(RuntimeError, match="scale"):
             ops.decode_attention_kv8(q, kp, vp, seqs, torch.zeros(1, dtype=torch.int32, device=DEV), pl, scale)
+
+
+@pytest.mark.parametrize("which", ["k", "v"])
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+def test_a_window_that_leaves_a_block_leaves_what_it_holds(which, QH, KH, D):
+    # rows 7 to 12 see nothing of the 10-token segment before them, though their window ends in its block
+    P, pages = 64, 12
+    kp, vp = random_pages(pages, KH, P, D, "int8", 47), random_pages(pages, KH, P, D, "int8", 48)
+    seqs, pl, T = layout([(64, [10, 64]), (40, [75, 40])], P, pages, flags=(8 << 8) | (1 << 24))
+    for e in (int(pl[0]), int(pl[3])):
+        (kp if which == "k" else vp).bytes[e, 0, 0] = 255
+    q = torch.randn(T, QH, D, device=DEV).bfloat16()
+    want, _ = ref.segmented_attention_kv8(q, kp, vp, seqs, pl, 0.1, torch.float64)
+    out = ops.prefill_attention_kv8(q, kp, vp, seqs, blocks_of(seqs), pl, 0.1)
+    assert torch.equal(torch.isnan(out.double()), torch.isnan(want))
+    assert bool(torch.isnan(out[:7]).any(dim=1).all()) and not bool(torch.isnan(out[7:64]).any())
