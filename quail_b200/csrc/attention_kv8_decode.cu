@@ -48,7 +48,6 @@ namespace {
 
 constexpr int kTile = 32;             // keys of a stage: two exponent blocks
 constexpr int kHeads = 8;             // query heads of one KV head per item
-constexpr int kMaxRows = 4096;        // sequences of one launch (their prefix sums are in shared memory)
 
 template <int D>
 struct DecGeom {
@@ -59,6 +58,12 @@ struct DecGeom {
   static constexpr int kRing = kWarps * kStages * kStageBytes;
   static constexpr int kBlocksPerSm = D == 64 ? 5 : D == 128 ? 3 : 1;
   static constexpr int kPartial = kHeads * D + 2 * kHeads;     // floats of a partial result: O, m, l
+  static constexpr int kFixed = kRing + kWarps * kKv8MaxSeg * 16 + 32;
+  // Sequences of one launch: their prefix sums are in shared memory, beside which kBlocksPerSm CTAs still have to
+  // fit (228 KB an SM, 1 KB of each CTA's reserved), as the ranges are made for one wave. head_dim 128: 2743.
+  static constexpr int kFit = (233472 / kBlocksPerSm - 1024 - kFixed) / 4 - 1;
+  static constexpr int kMaxRows = kFit < 4096 ? kFit : 4096;
+  static_assert(kBlocksPerSm * (kFixed + (kMaxRows + 1) * 4 + 1024) <= 233472, "a full launch keeps its CTAs an SM");
 };
 
 __device__ __forceinline__ uint32_t movm(uint32_t x) {
@@ -865,12 +870,11 @@ template <int D, bool FP8, bool MX, bool SMALL, bool ITEM>
 static void launch_decode_p(const Kv8Attn& a, int n, cudaStream_t st, int dev, const torch::Tensor& like) {
   using Gm = DecGeom<D>;
   constexpr int kMinTiles = 2;
-  constexpr int kFixed = Gm::kRing + Gm::kWarps * kKv8MaxSeg * 16 + 32;
-  const int smem = kFixed + (n + 1) * 4;
+  const int smem = Gm::kFixed + (n + 1) * 4;
   static bool configured[64] = {false};
   if (!configured[dev]) {
     C10_CUDA_CHECK(cudaFuncSetAttribute(decode_kv8_kernel<D, FP8, MX, SMALL, ITEM>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                        kFixed + (kMaxRows + 1) * 4));
+                                        Gm::kFixed + (Gm::kMaxRows + 1) * 4));
     configured[dev] = true;
   }
   if constexpr (ITEM) {
@@ -935,9 +939,11 @@ void decode_attention_kv8(const torch::Tensor& q, const torch::Tensor& kc, const
   const int D = (int)q.size(2);
   // the tiles of a launch are counted in 32 bits: a row has at most 4 times the page list's
   const int64_t row_tiles = kKv8MaxSeg * ((int64_t)a.n_list * a.P / kTile + 1);
-  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(kMaxRows, INT32_MAX / row_tiles));
-  for (int first = 0; first < total; first += most) {
-    const int n = std::min(most, total - first);
+  const int fit = D == 64 ? DecGeom<64>::kMaxRows : D == 128 ? DecGeom<128>::kMaxRows : DecGeom<256>::kMaxRows;
+  const int most = (int)std::max<int64_t>(1, std::min<int64_t>(fit, INT32_MAX / row_tiles));
+  const int launches = (total + most - 1) / most, each = (total + launches - 1) / launches;
+  for (int first = 0; first < total; first += each) {
+    const int n = std::min(each, total - first);
     a.blocks = dseqs.data_ptr<int>() + first;
 #define QB_DEC8(DD)                                                                                     \
   if (D == DD) {                                                                                        \

@@ -155,3 +155,16 @@ def test_a_window_that_leaves_a_block_leaves_what_it_holds(which, QH, KH, D):
     out = ops.prefill_attention_kv8(q, kp, vp, seqs, blocks_of(seqs), pl, 0.1)
     assert torch.equal(torch.isnan(out.double()), torch.isnan(want))
     assert bool(torch.isnan(out[:7]).any(dim=1).all()) and not bool(torch.isnan(out[7:64]).any())
+
+
+def test_decode_of_more_rows_than_one_launch_takes():
+    P, QH, KH, D, n = 16, 4, 1, 128, 2900
+    specs = [(1, [1 + (7 * i) % 37]) for i in range(n)]
+    pages = sum(-(-ln // P) for _, (ln,) in specs)
+    kp, vp = random_pages(pages, KH, P, D, "int8", 49), random_pages(pages, KH, P, D, "int8", 50)
+    seqs, pl, T = layout(specs, P, pages)
+    q = torch.randn(T, QH, D, device=DEV).bfloat16()
+    dseqs = torch.randperm(n, device=DEV).int()
+    lse = torch.empty(T, QH, device=DEV)
+    out = ops.decode_attention_kv8(q, kp, vp, seqs, dseqs, pl, 0.1, lse=lse)
+    check_rows(out, lse, q, kp, vp, seqs, pl, 0.1)
