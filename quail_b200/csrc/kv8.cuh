@@ -154,15 +154,16 @@ __device__ __forceinline__ void kv8_load_seq(Kv8Seq& s, const Kv8Attn& a, int se
   s.win = (v[3] >> 8) & 0xffff;
   s.win_all = (v[3] >> 24) & 1;
   const int pshift = __ffs(a.P) - 1;
+  bool bad = false;
 #pragma unroll
   for (int i = 0; i < kKv8MaxSeg; ++i) {
     s.len[i] = i < s.nseg ? max(v[4 + i], 0) : 0;
     s.off[i] = v[4 + kKv8MaxSeg + i];
-    if (s.len[i] > 0 && (s.off[i] < 0 || (s.len[i] - 1) >> pshift >= a.n_list - s.off[i])) {
-      kv8_error(a.err, kErrBadShape);
-      s.len[i] = 0;
-    }
+    const bool past = s.len[i] > 0 && (s.off[i] < 0 || (s.len[i] - 1) >> pshift >= a.n_list - s.off[i]);
+    if (past) s.len[i] = 0;
+    bad |= past;
   }
+  if (bad) kv8_error(a.err, kErrBadShape);
   s.own_len = 0;
   s.before = 0;
 #pragma unroll
