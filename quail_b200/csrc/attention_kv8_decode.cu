@@ -905,13 +905,15 @@ static void launch_decode_p(const Kv8Attn& a, int n, cudaStream_t st, int dev, c
 }
 
 template <int D, bool FP8, bool MX>
-static void launch_decode(const Kv8Attn& a, int n, cudaStream_t st, int dev, const torch::Tensor& like) {
-  // A CTA per item where they are one wave of CTAs at most and short: by the page list's length (a bound
-  // of the keys, and all the host knows) at most 1024 keys a sequence on average. Eight rows of ~230 keys:
-  // 10.3 us so, 16.5 us as equal ranges and a join; a long row would be 8 CTAs' work so.
+static void launch_decode(const Kv8Attn& a, int n, bool few_keys, cudaStream_t st, int dev,
+                          const torch::Tensor& like) {
+  // A CTA per item where they are one wave of CTAs at most and no row has many keys (ops/kv8.py says what the
+  // caller knows of that): a row of 1000 keys is 8 tiles for each of its CTA's warps. 32 query and 8 KV heads of
+  // 128, in us, so and as equal ranges with a join: 8 rows of 230 keys 13.2, 21.4; of 1000 keys 20.5, 25.6; 55 rows
+  // of 1000 keys 37.8, 48.1; but a row of 2000 keys among 7 of 100 29.5, 23.6; of 4000 keys 49.2, 25.6.
   const int G = a.QH / a.KH;
   const int64_t items = (int64_t)n * a.KH * ((G + kHeads - 1) / kHeads);
-  const bool item = items <= (int64_t)num_sms(dev) * DecGeom<D>::kBlocksPerSm && (int64_t)a.n_list * a.P <= (int64_t)n * 1024;
+  const bool item = few_keys && items <= (int64_t)num_sms(dev) * DecGeom<D>::kBlocksPerSm;
   if (item)
     a.P < kTile ? launch_decode_p<D, FP8, MX, true, true>(a, n, st, dev, like)
                 : launch_decode_p<D, FP8, MX, false, true>(a, n, st, dev, like);
@@ -920,12 +922,12 @@ static void launch_decode(const Kv8Attn& a, int n, cudaStream_t st, int dev, con
                 : launch_decode_p<D, FP8, MX, false, false>(a, n, st, dev, like);
 }
 
-// dseqs [n] int32: the sequences whose last query token is read
+// dseqs [n] int32: the sequences whose last query token is read; few_keys: none of them has many keys (a hint)
 void decode_attention_kv8(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& kb,
                           const torch::Tensor& vc, const torch::Tensor& vb, const torch::Tensor& seqs,
                           const torch::Tensor& dseqs, const torch::Tensor& page_list, double scale,
                           torch::Tensor& out, const c10::optional<torch::Tensor>& out_sf,
-                          const c10::optional<torch::Tensor>& lse) {
+                          const c10::optional<torch::Tensor>& lse, bool few_keys) {
   const char* what = "decode_attention_kv8";
   Kv8Attn a = kv8_args(what, q, kc, kb, vc, vb, seqs, page_list, scale, out, out_sf, lse);
   TORCH_CHECK(dseqs.scalar_type() == at::kInt && dseqs.is_contiguous() && dseqs.device() == q.device(), what,
@@ -948,9 +950,11 @@ void decode_attention_kv8(const torch::Tensor& q, const torch::Tensor& kc, const
 #define QB_DEC8(DD)                                                                                     \
   if (D == DD) {                                                                                        \
     if (fp8)                                                                                            \
-      mx ? launch_decode<DD, true, true>(a, n, st, dev, q) : launch_decode<DD, true, false>(a, n, st, dev, q); \
+      mx ? launch_decode<DD, true, true>(a, n, few_keys, st, dev, q)                                    \
+         : launch_decode<DD, true, false>(a, n, few_keys, st, dev, q);                                  \
     else                                                                                                \
-      mx ? launch_decode<DD, false, true>(a, n, st, dev, q) : launch_decode<DD, false, false>(a, n, st, dev, q); \
+      mx ? launch_decode<DD, false, true>(a, n, few_keys, st, dev, q)                                   \
+         : launch_decode<DD, false, false>(a, n, few_keys, st, dev, q);                                 \
   }
     QB_DEC8(64)
     QB_DEC8(128)

@@ -133,7 +133,7 @@ void decode_attention_kv8(const torch::Tensor& q, const torch::Tensor& kc, const
                           const torch::Tensor& vc, const torch::Tensor& vb, const torch::Tensor& seqs,
                           const torch::Tensor& dseqs, const torch::Tensor& page_list, double scale,
                           torch::Tensor& out, const c10::optional<torch::Tensor>& out_sf,
-                          const c10::optional<torch::Tensor>& lse);
+                          const c10::optional<torch::Tensor>& lse, bool few_keys);
 
 static std::mutex g_err_mu;
 static int* g_err[64] = {nullptr};

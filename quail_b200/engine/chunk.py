@@ -74,6 +74,7 @@ class Chunk:
     final_rows: torch.Tensor
     readout_tags: list = field(default_factory=list)
     dseqs: torch.Tensor | None = None
+    dkeys: int | None = None    # the most keys one of dseqs' rows reads (None: not known)
     state_io: torch.Tensor | None = None
     blocks: torch.Tensor | None = None
     num_seqs: int = 0
@@ -158,7 +159,7 @@ class ChunkPacker:
             host["tree"] = tree
         return Chunk(num_tokens=n_tok, ids=views[0], positions=views[1], slots=views[2],
                      seqs=views[3].view(-1, SEQ_INTS), tiles=views[4].view(-1, 2), page_list=views[5],
-                     final_rows=views[6], dseqs=views[7], state_io=views[8].view(-1, 2),
+                     final_rows=views[6], dseqs=views[7], dkeys=host["dkeys"], state_io=views[8].view(-1, 2),
                      blocks=views[9].view(-1, 2), readout_tags=tags, tree=tree_dev, rope3=rope3,
                      num_seqs=len(specs), host=host, upload_bytes=up,
                      full_readout=any(s.full and s.readout for s in specs),
@@ -183,6 +184,7 @@ class ChunkPacker:
         tiles: list[int] = []
         blocks: list[tuple] = []      # (keys read, sequence, first token)
         dseqs: list[int] = []
+        dkeys = 0
         final_rows: list[int] = []
         tags: list = []
         split = self.split_decode
@@ -228,6 +230,9 @@ class ChunkPacker:
             seqs += row
             if n == 1 and split:
                 dseqs.append(si)
+                keys = own_len + sum(ln for _, ln in reads)
+                if keys > dkeys:
+                    dkeys = keys
             else:
                 for q0 in range(0, n, ATTN_BLOCK_Q):
                     tiles += (si, q0)
@@ -248,7 +253,7 @@ class ChunkPacker:
                 "slots": np.asarray(slots, dtype=i32), "seqs": np.asarray(seqs, dtype=i32).reshape(S, SEQ_INTS),
                 "tiles": np.asarray(tiles, dtype=i32).reshape(-1, 2), "page_list": np.asarray(page_list, dtype=i32),
                 "final_rows": np.asarray(final_rows, dtype=i32), "dseqs": np.asarray(dseqs, dtype=i32),
-                "state_io": sio,
+                "state_io": sio, "dkeys": dkeys,
                 "blocks": np.asarray([(b[1], b[2]) for b in sorted(blocks, key=lambda b: -b[0])],
                                      dtype=i32).reshape(-1, 2)}
         return host, tags

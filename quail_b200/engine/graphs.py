@@ -16,7 +16,9 @@ token count (buckets 8, 16, 32, 64, 128, 256, 512, 1024):
     not written back)), copies it with one H2D copy and replays the graph;
   * the first pass of a bucket runs eagerly (its result is the pass's) and
     then captures; a page list longer than the bucket's capacity recaptures
-    with twice the capacity; new answer rows (another query) drop the graphs.
+    with twice the capacity; new answer rows (another query) drop the graphs;
+    over 8-bit pages a bucket has one graph for passes whose rows have few
+    keys and one for the others (their decode attention differs).
 
 Every bucket's graph allocates from one shared memory pool (they replay one
 at a time on one stream), and the logits a replay returns live in that pool
@@ -58,14 +60,14 @@ class _Entry:
         self.out = None
         self.launches = 0
 
-    def chunk(self, full: bool, topk: bool = False) -> Chunk:
+    def chunk(self, full: bool, topk: bool = False, dkeys: int | None = None) -> Chunk:
         v, o = {}, 0
         for k in PARTS:
             v[k] = self.buf[o:o + self.sizes[k]]
             o += self.sizes[k]
         return Chunk(num_tokens=self.B, ids=v["ids"], positions=v["positions"], slots=v["slots"],
                      seqs=v["seqs"].view(-1, SEQ_INTS), tiles=v["tiles"].view(-1, 2), page_list=v["page_list"],
-                     final_rows=v["final_rows"], dseqs=v["dseqs"], state_io=v["state_io"].view(-1, 2),
+                     final_rows=v["final_rows"], dseqs=v["dseqs"], dkeys=dkeys, state_io=v["state_io"].view(-1, 2),
                      blocks=v["blocks"].view(-1, 2), num_seqs=self.B, full_readout=full, topk=topk)
 
     def fill(self, host: dict) -> int:
@@ -149,17 +151,22 @@ class DecodeGraphs:
             self.entries.clear()
             self._rows_key = key
         pl_need = host["page_list"].size
-        e = self.entries.get((B, full, topk))
+        # the 8-bit cache's decode has a variant for rows of few keys: a graph is captured for one of them
+        dkeys = None
+        if self.arena.kv8:
+            dkeys = ops.KV8_FEW_KEYS if host["dkeys"] <= ops.KV8_FEW_KEYS else ops.KV8_FEW_KEYS + 1
+        at = (B, full, topk, dkeys)
+        e = self.entries.get(at)
         if e is not None and pl_need > e.pl_cap:
             e = None
         if e is None:
             cap = 1 << max(10, int(np.ceil(np.log2(max(pl_need, 1)))) + 1)
             e = _Entry(B, cap, self.device)
-            self.entries[(B, full, topk)] = e
+            self.entries[at] = e
         nbytes = e.fill(host)
         R = host["final_rows"].size
         if e.graph is None:
-            chunk = e.chunk(full, topk)
+            chunk = e.chunk(full, topk, dkeys)
             out = self.model.forward_chunk(chunk, self.arena)      # eager: this pass's answer
             torch.cuda.current_stream().synchronize()
             n0 = ops.launch_count()

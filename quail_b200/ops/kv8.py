@@ -21,6 +21,7 @@ from quail_b200.ops import kernels as K
 KV8_BLOCK = 16                            # tokens that share an exponent byte
 KV8_DTYPES = {"int8": torch.int8, "fp8": torch.float8_e4m3fn}
 KV8_HEAD_DIMS = frozenset({64, 128, 256})
+KV8_FEW_KEYS = 1024                       # up to this many keys a row, few rows take a CTA per row and KV head
 
 
 class Pages8:
@@ -131,18 +132,34 @@ def prefill_attention_kv8(q, k_pages: Pages8, v_pages: Pages8, seqs, blocks, pag
     return (out, out_scale) if fp8_out else out
 
 
+def _few_keys(rows: int, listed: int, page_tokens: int, max_keys: int | None) -> bool:
+    """Whether no row of a decode has many keys, by what the host knows.
+
+    Without `max_keys`, by the page list: every other row has a page of its own in it, so one row
+    reads the rest of it at most. That bound is several times what most rows have, so it may be
+    four times as large: the worst case, one row of 4000 keys among short ones, takes 49 us for
+    26, while 8 to 30 short rows take 11 to 20 us for 19 to 27.
+    """
+    if max_keys is not None:
+        return max_keys <= KV8_FEW_KEYS
+    return (listed - rows + 1) * page_tokens <= 4 * KV8_FEW_KEYS
+
+
 def decode_attention_kv8(q, k_pages: Pages8, v_pages: Pages8, seqs, dseqs, page_list, softmax_scale: float, *,
-                         fp8_out: bool = False, out=None, out_scale=None, lse=None):
+                         fp8_out: bool = False, out=None, out_scale=None, lse=None, max_keys: int | None = None):
     """Attention of the last query token of the sequences dseqs int32 [n] over the 8-bit cache.
 
-    Outputs as prefill_attention_kv8; only those tokens' rows are written.
+    Outputs as prefill_attention_kv8; only those tokens' rows are written. `max_keys`: the most
+    keys one of the rows reads, where the caller knows it. It changes the time and the order of
+    fp32 sums, not what is computed.
     """
     _check_heads("decode_attention_kv8", q, k_pages)
     out, out_scale = _outputs(q, fp8_out, out, out_scale)
     if dseqs.numel():
         K.count_launch()
         K.native().decode_attention_kv8(q, k_pages.codes, k_pages.bytes, v_pages.codes, v_pages.bytes, seqs, dseqs,
-                                        page_list, softmax_scale, out, out_scale, lse)
+                                        page_list, softmax_scale, out, out_scale, lse,
+                                        _few_keys(dseqs.numel(), page_list.numel(), k_pages.page_tokens, max_keys))
     return (out, out_scale) if fp8_out else out
 
 
@@ -191,14 +208,15 @@ def chunk_attention_kv8(q, k_pages: Pages8, v_pages: Pages8, chunk, softmax_scal
     log-sum-exps, as there."""
     T, QH, D = q.shape
     tree = getattr(chunk, "tree", None)
-    dseqs = getattr(chunk, "dseqs", None)
+    dseqs, dkeys = getattr(chunk, "dseqs", None), getattr(chunk, "dkeys", None)
     if tree is not None and chunk.tiles.shape[0] > 0:
         o_a = torch.empty(T, QH * D, dtype=torch.bfloat16, device=q.device)
         lse_a = torch.empty(T, QH, dtype=torch.float32, device=q.device)
         prefill_attention_kv8(q, k_pages, v_pages, tree["seqs_a"], tree["blocks_a"], chunk.page_list, softmax_scale,
                               out=o_a, lse=lse_a)
         if dseqs is not None:
-            decode_attention_kv8(q, k_pages, v_pages, chunk.seqs, dseqs, chunk.page_list, softmax_scale, out=o_a)
+            decode_attention_kv8(q, k_pages, v_pages, chunk.seqs, dseqs, chunk.page_list, softmax_scale, out=o_a,
+                                 max_keys=dkeys)
         rows = tree["rows"]
         o_b = torch.empty(rows.numel(), QH * D, dtype=torch.bfloat16, device=q.device)
         lse_b = torch.empty(rows.numel(), QH, dtype=torch.float32, device=q.device)
@@ -211,5 +229,5 @@ def chunk_attention_kv8(q, k_pages: Pages8, v_pages: Pages8, chunk, softmax_scal
                               fp8_out=mx, out=out, out_scale=out_scale)
     if dseqs is not None:
         decode_attention_kv8(q, k_pages, v_pages, chunk.seqs, dseqs, chunk.page_list, softmax_scale, fp8_out=mx,
-                             out=out, out_scale=out_scale)
+                             out=out, out_scale=out_scale, max_keys=dkeys)
     return (out, out_scale) if mx else out

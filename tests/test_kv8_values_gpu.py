@@ -168,3 +168,19 @@ def test_decode_of_more_rows_than_one_launch_takes():
     lse = torch.empty(T, QH, device=DEV)
     out = ops.decode_attention_kv8(q, kp, vp, seqs, dseqs, pl, 0.1, lse=lse)
     check_rows(out, lse, q, kp, vp, seqs, pl, 0.1)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("QH,KH,D", GEOMETRIES)
+def test_decode_gives_the_same_whatever_is_said_of_its_rows(kind, QH, KH, D):
+    # a hint that is too small or too large changes the time only; a long row among short ones, a padded list
+    P, pages = 16, 250
+    kp, vp = random_pages(pages, KH, P, D, kind, 51), random_pages(pages, KH, P, D, kind, 52)
+    seqs, pl, T = layout([(1, [48, 30]), (1, [48, 2500]), (1, [48, 1]), (1, [48, 600])], P, pages, prefix_shared=True)
+    q = torch.randn(T, QH, D, device=DEV).bfloat16()
+    dseqs = torch.arange(4, dtype=torch.int32, device=DEV)
+    for table in (pl, torch.cat([pl, pl.new_zeros(5000)])):
+        for most in (None, 1, 2548, 1 << 40):
+            lse = torch.empty(T, QH, device=DEV)
+            out = ops.decode_attention_kv8(q, kp, vp, seqs, dseqs, table, 0.1, lse=lse, max_keys=most)
+            check_rows(out, lse, q, kp, vp, seqs, pl, 0.1)
