@@ -8,6 +8,8 @@ row:
 
   first call   one task: reads the shared instruction prefix, writes the
                document + the call's question, reads out the last token.
+               Over 8-bit pages (an exponent for 16 tokens) the document is a
+               task alone and its first call follows it like the next ones.
   next calls   one task each: reads the prefix and the first task's document
                tokens (borrowed pages), writes only its own question.
                Consecutive non-filter calls run side by side; a filter
@@ -150,6 +152,11 @@ class RegionRun:
         # is recomputed (a replay)
         self.retain_key = None
         self._resident_doc = [False] * len(docs)
+        # over 8-bit pages a document's pages hold its own tokens only, and its first question too has
+        # pages of its own: a question's tokens in the document's last block would coarsen that block's
+        # exponent (or mark it, if they are not finite) for every later question
+        self.apart = bool(getattr(getattr(executor, "arena", None), "kv8", False))
+        self._doc_rows: dict = {}             # row -> its document's readout rows (a max-pooled first call, apart)
         # columns after the answer rows in a full readout: argmax, lse
         self.nans = answer_width
 
@@ -223,6 +230,8 @@ class RegionRun:
         elif call.kind in ("map", "extract"):
             self._decode_step(r, ci, row, [])
         elif call.kind == "features":
+            if ci == 0 and r in self._doc_rows:
+                row = np.concatenate([self._doc_rows.pop(r), np.asarray(row)])
             res.values[call.name] = feature_list(row)
             self._finish_call(r, ci)
         self.asked += 1
@@ -511,6 +520,7 @@ class RegionRun:
         self.fresh_tokens += P
         self.ex.submit(Task(np_rows=True, key=PREFIX_KEY, tokens=self.prefix, pos_start=0, free_after=False))
         first = self.calls[0]
+        self._leave = self._follow_pages() if self.apart else 0
         pinned, cap = 0, self.ex.pool.num_pages // 2
         # a first call that reads every own token (max-pooled features) needs the document computed
         reusable = not (first.kind == "features" and first.pooling == "max")
@@ -541,8 +551,11 @@ class RegionRun:
                     continue
                 self.fresh_tokens += len(doc)
                 self.ex.submit(Task(np_rows=True, key=("doc", r), tokens=doc, pos_start=P,
-                                    reads=[(PREFIX_KEY, P)], free_after=False,
+                                    reads=[(PREFIX_KEY, P)], free_after=False, leave_pages=self._leave,
                                     on_done=lambda t, row, r=r: self._doc_only(r)))
+                continue
+            if self.apart and len(doc):
+                self._submit_apart(r, doc, first)
                 continue
             toks = np.concatenate([doc, first.suffix])
             self.fresh_tokens += len(toks)
@@ -553,6 +566,30 @@ class RegionRun:
                                 topk=first.copy,
                                 readout_rows=self._pooled_rows(first, len(toks)),
                                 on_done=lambda t, row, r=r: self._answered(r, 0, row), free_after=False))
+
+    def _submit_apart(self, r: int, doc, first: Call) -> None:
+        """Row r's document alone; its questions follow it, the first one too."""
+        self._resident_doc[r] = True
+        self._next[r] = 0
+        self._pending[r] = 1
+        self.fresh_tokens += len(doc)
+        rows = tuple(range(len(doc))) if first.kind == "features" and first.pooling == "max" else None
+
+        def done(task, got, r=r):
+            if rows is not None:
+                self._doc_rows[r] = np.array(got)
+            self._doc_only(r)
+        self.ex.submit(Task(np_rows=True, key=("doc", r), tokens=doc, pos_start=len(self.prefix),
+                            reads=[(PREFIX_KEY, len(self.prefix))], free_after=False, readout=rows is not None,
+                            readout_rows=rows, on_done=done, leave_pages=self._leave))
+
+    def _follow_pages(self) -> int:
+        """Pages that stay free for questions when a document is admitted: a quarter of the arena (about as many
+        questions as documents are then in flight), at least what one call of a row holds at a time."""
+        need = self.ex.pool.pages_needed
+        one = max(need(len(c.suffix) + self._reserve(c)) + sum(need(len(lab) - 1) for lab in c.labels)
+                  for c in self.calls)
+        return max(self.ex.pool.num_pages // 4, one)
 
     def _doc_only(self, r: int) -> None:
         self._pending[r] = 0

@@ -61,6 +61,7 @@ class Task:
     full_readout: bool = False                       # also argmax / log-sum-exp over the vocabulary
     topk: bool = False                               # and the top-k token ids and logits
     reserve_tokens: int = 0                          # decode headroom allocated with the key's pages
+    leave_pages: int = 0                             # pages that stay free when the key is admitted among others
     got_rows: list = field(default_factory=list)     # readout rows of the pieces already collected
     np_rows: bool = False                            # on_done gets numpy rows (views of the pass's host copy)
     # a document-isolated block: its own tokens read each other both ways, so it runs in one
@@ -250,6 +251,15 @@ class StageExecutor:
                     deferred.append(task)
                     continue
                 cap = total + (task.reserve_tokens if self.answer_headroom else 0)
+                if task.leave_pages and (specs or self._inflight or self.follow or self.cont):
+                    # the keys in flight need the pages left to finish and free theirs
+                    want = self.pool.pages_needed(cap) + task.leave_pages
+                    if self.pool.free_pages < want:
+                        self._evict(want)
+                    if self.pool.free_pages < want:
+                        deferred.append(task)
+                        no_new = True
+                        continue
                 pages = self.pool.alloc(task.key, total, cap)
                 if pages is None:
                     self._evict(self.pool.pages_needed(cap))
