@@ -329,10 +329,11 @@ class RegionRun:
 
     def _draft(self, r, ci, room: int) -> tuple:
         """Document-copy draft: when the copy so far continues at one document position only,
-        the next few document tokens, to verify in one pass (reference: extract/candidates.py)."""
+        the next few document tokens, to verify in one pass (reference: extract/candidates.py).
+        Not over 8-bit pages: a rejected token would have coarsened its block for the accepted ones."""
         state = self._copies.get((r, ci))
         doc = self.docs[r]
-        if state is None or state.size != 1 or state[0] >= len(doc):
+        if self.apart or state is None or state.size != 1 or state[0] >= len(doc):
             return ()
         p = int(state[0])
         n = min(DRAFT_TOKENS, room, len(doc) - p)

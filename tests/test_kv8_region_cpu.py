@@ -138,3 +138,14 @@ def test_many_documents_in_a_small_arena_leave_room_for_their_questions():
     assert all("a" in r.values for r in got.results) and ex.pool.free_pages == ex.pool.num_pages
     got = run(ex, docs, [score("a", [3, 4]), score("b", [9])])
     assert all("b" in r.values for r in got.results)
+
+
+def test_no_copy_drafts_over_8_bit_pages():
+    # a draft's rejected tokens share blocks with the tokens before them
+    doc = DOCS[3]
+    call = Call(kind="extract", suffix=np.asarray([3], np.int32), copy=True, name="x")
+    for kind, want in (("int8", ()), (None, tuple(int(t) for t in doc[2:6]))):
+        arena = KVArena(1, 64, P, KH, D, device="cpu", dtype=KV8_DTYPES[kind] if kind else torch.float32)
+        r = RegionRun(StageExecutor(Stub(6), arena, 256), np.arange(1, 20, dtype=np.int32), [doc], [call], answer_width=4)
+        r._copies[(0, 0)] = np.asarray([2])
+        assert r._draft(0, 0, 4) == want
