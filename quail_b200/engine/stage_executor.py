@@ -35,6 +35,7 @@ import torch
 
 from quail_b200.engine.arena import ArenaFullError
 from quail_b200.engine.chunk import ChunkPacker, SeqSpec
+from quail_b200.ops.kv8 import KV8_BLOCK
 
 
 class OversizedDocumentError(ArenaFullError):
@@ -123,6 +124,7 @@ class StageExecutor:
         self.pool = arena.pool
         self.chunk_tokens = chunk_tokens
         self.min_piece = min_piece
+        self.piece_tokens = KV8_BLOCK if getattr(arena, "kv8", False) else 1   # a piece of a prompt ends at a multiple
         self.max_seqs = max_seqs
         # continuations (decode steps) per pass: with more decoding rows than this they
         # split into groups that alternate, so the host builds one group's next step
@@ -281,6 +283,16 @@ class StageExecutor:
                         stop = True
                         break
             piece = min(task.remaining, room)
+            if piece < task.remaining and self.piece_tokens > 1:
+                # a piece ends where a block of the cache does, so that what the block holds does not
+                # depend on how its tokens came to be split
+                over = (task.own_prefix + task.done + piece) % self.piece_tokens
+                if over < piece:
+                    piece -= over
+                elif specs:
+                    deferred.append(task)
+                    stop = True
+                    break
             if task.bidirectional and piece < task.remaining:
                 if task.remaining > self.chunk_tokens:
                     raise OversizedDocumentError(

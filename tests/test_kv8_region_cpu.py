@@ -149,3 +149,21 @@ def test_no_copy_drafts_over_8_bit_pages():
         r = RegionRun(StageExecutor(Stub(6), arena, 256), np.arange(1, 20, dtype=np.int32), [doc], [call], answer_width=4)
         r._copies[(0, 0)] = np.asarray([2])
         assert r._draft(0, 0, 4) == want
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+@pytest.mark.parametrize("chunk_tokens", [17, 70, 100])
+def test_pieces_of_a_document_end_where_a_block_does(kind, chunk_tokens):
+    # a block written in two pieces would be rounded twice, by where the piece happened to end
+    ex = executor(kind, chunk_tokens=chunk_tokens)
+    docs = [*DOCS, np.asarray([LOUD if j % 11 == 10 else j % 50 + 1 for j in range(90)], np.int32)]
+    run(ex, docs, [score("a", [3, 4])])
+    assert max(ex.stats.pass_tokens) <= chunk_tokens and ex.stats.passes > len(docs) // 2
+    for i, doc in enumerate(docs):
+        assert all(torch.equal(x, y) for x, y in zip(held(ex, ("kept", i), doc), alone(doc, kind)))
+
+
+def test_a_pass_smaller_than_a_block_still_gets_on():
+    ex = executor(chunk_tokens=5)
+    got = run(ex, DOCS, [score("a", [3, 4])], retain=False)
+    assert all("a" in r.values for r in got.results)
