@@ -115,8 +115,9 @@ class Budgets:
         if pages < need:
             raise MemoryError(f"the arena holds {pages} pages; a chunk of {self.chunk_tokens} tokens needs {need}")
         # enough for eight chunks in flight and retained documents; more
-        # only costs start-up time zeroing memory nothing reads
-        pages = min(pages, 8 * (self.chunk_tokens // page_tokens) + 256)
+        # only costs start-up time zeroing memory nothing reads. The bound is one
+        # of memory: as many bytes of 8-bit pages hold about twice the tokens
+        pages = min(pages, int((8 * (self.chunk_tokens // page_tokens) + 256) * 2 / value))
         cap = kv_pool_cap_tokens()
         if cap is not None:
             # an experiment's cap on the KV pool (the reference's QUAIL_KV_POOL_TOKENS,

@@ -31,3 +31,20 @@ def test_a_row_written_before_kept_rows_of_its_block_leaves_their_values(kind):
     want = torch.ones(16, 2, 64, dtype=torch.float64)
     want[3] = 8
     assert torch.equal(ref.kv8_values(p.codes, p.bytes)[0], want)
+
+
+@pytest.mark.parametrize("name,device,chunk", [("qwen3-4b-fp8", "b200", None), ("qwen3-8b-bf16", "b200", None),
+                                               ("qwen3-32b-fp8", "b200", None), ("qwen3-4b-fp8", "b200", 65_536),
+                                               ("qwen3-32b-fp8", "h100-sxm", 65_536), ("qwen3-tiny", "cpu", None)])
+def test_the_engines_arena_of_8_bit_pages_holds_twice_the_tokens(name, device, chunk, monkeypatch):
+    from quail_b200.models.config import MODEL_CONFIGS
+    from quail_b200.planner.budgets import Budgets
+    monkeypatch.delenv("QUAIL_KV_POOL_TOKENS", raising=False)
+    cfg = MODEL_CONFIGS[name]
+
+    def pages(kv):
+        return Budgets.for_model(cfg, device, chunk_tokens=chunk, kv_dtype=kv).arena_pages(128)
+    # a byte and 1/16 of one per head_dim values against two, both rounded down to whole pages
+    ratio = 2 / (1 + 1 / (16 * cfg.head_dim))
+    for kind in ("int8", "fp8"):
+        assert abs(pages(kind) - ratio * pages("bf16")) <= ratio + 1
