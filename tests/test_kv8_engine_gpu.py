@@ -39,3 +39,64 @@ def test_decode_graphs_hold_the_form_for_few_keys_and_the_other():
         assert (graphs.captures, graphs.replays) == ((1, step) if step < 2 else (2, step - 1))
     assert sorted(at[3] for at in graphs.entries) == [ops.KV8_FEW_KEYS, ops.KV8_FEW_KEYS + 1]
     assert ops.read_and_clear_error(0) == 0
+
+
+def session(kind, **kw):
+    import pyarrow as pa
+
+    import quail_b200 as quail
+    rng = np.random.default_rng(0)
+    words = ["ending", "music", "cast", "plot", "money", "great", "bad", "long"]
+    bodies = [" ".join(rng.choice(words, size=int(rng.integers(3, 40)))) for _ in range(40)]
+    s = quail.Session(config=quail.EngineConfig(model="qwen3-gpu-tiny-gqa4", device="b200", chunk_tokens=2048,
+                                                kv_dtype=kind, **kw))
+    s.register("t", pa.table({"id": list(range(40)), "body": bodies}))
+    return s, bodies
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_sessions_answer_every_kind_of_call(kind):
+    s, bodies = session(kind)
+    with s:
+        t = s.sql("""
+            SELECT id, AI.SCORE(PROMPT('Positive? {0}', body)) AS s,
+                   AI.CLASSIFY(body, ['praise', 'complaint'], {'probabilities': true}) AS k,
+                   AI.MAP(body, 'Summarize.', 4) AS m, AI.EXTRACT(body, ['What is it about?']) AS e
+            FROM t ORDER BY id""").collect()
+        kept = s.sql("SELECT id FROM t WHERE AI.IF(PROMPT('Is it about music? {0}', body)) ORDER BY id").collect()
+        flags = s.sql("SELECT id, AI.IF(PROMPT('Is it about music? {0}', body)) AS f FROM t ORDER BY id").collect()
+        assert s.engine().executor.stats.reused >= 40
+    assert t.num_rows == 40 and all(0.0 < x < 1.0 for x in t.column("s").to_pylist())
+    assert set(t.column("k").to_pylist()) <= {"praise", "complaint"}
+    assert all(isinstance(m, str) for m in t.column("m").to_pylist())
+    for body, e in zip(bodies, t.column("e").to_pylist()):
+        assert all(x is None or x.strip() in body for x in e)
+    want = [i for i, f in zip(flags.column("id").to_pylist(), flags.column("f").to_pylist()) if f]
+    assert kept.column("id").to_pylist() == want
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_retained_documents_are_the_same_whatever_was_asked(kind):
+    asked = ("SELECT id, AI.IF(PROMPT('Would somebody who wrote this go again? {0}', body)) AS m FROM t ORDER BY id",
+             "SELECT id, AI.IF(PROMPT('Is it about music? {0}', body)) AS f FROM t ORDER BY id")
+    held = []
+    for queries in (asked, asked[::-1], asked[1:]):
+        s, _ = session(kind)
+        with s:
+            for q in queries:
+                s.sql(q).collect()
+            arena = s.engine().arena
+            got = {}
+            for key in arena.pool.retained:
+                pages, n = arena.pool.owned[key], arena.pool.tokens[key]
+                parts = []
+                for i in range(arena.num_layers):
+                    for p in arena.layer(i):
+                        codes = torch.cat([p.codes[g].view(torch.uint8) for g in pages], dim=1)[:, :n]
+                        parts += [codes, torch.cat([p.bytes[g] for g in pages], dim=1)[:, :-(-n // 16)]]
+                got[key] = [x.cpu() for x in parts]
+            held.append(got)
+    assert len(held[0]) >= 35 and held[0].keys() == held[1].keys() == held[2].keys()
+    for other in held[1:]:
+        for key, parts in held[0].items():
+            assert all(torch.equal(x, y) for x, y in zip(parts, other[key]))
