@@ -232,6 +232,8 @@ class PagePool:
         """Give `key` its own page of token `tokens` and own pages after it, where forks share them, so that
         it may be rewound to `tokens` and written. Returns the [(source page, copy)] to copy, or None if
         the pool is short (nothing is changed then)."""
+        if not 0 <= tokens <= self.tokens[key]:
+            raise ValueError(f"{key!r} holds {self.tokens[key]} tokens, not {tokens}")
         have = self.owned[key]
         at = tokens // self.page_tokens
         shared = [i for i in range(at, len(have)) if self.owners[have[i]] > 1]

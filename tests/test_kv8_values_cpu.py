@@ -48,3 +48,16 @@ def test_the_engines_arena_of_8_bit_pages_holds_twice_the_tokens(name, device, c
     ratio = 2 / (1 + 1 / (16 * cfg.head_dim))
     for kind in ("int8", "fp8"):
         assert abs(pages(kind) - ratio * pages("bf16")) <= ratio + 1
+
+
+def test_unshare_refuses_a_place_the_key_does_not_have():
+    from quail_b200.engine.arena import PagePool
+    p = PagePool(8, 16)
+    p.alloc("p", 32)
+    assert p.fork("p", "c") == []
+    for tokens in (-1, 33):
+        with pytest.raises(ValueError, match="tokens"):
+            p.unshare("c", tokens)
+        p.check()
+    assert len(p.unshare("c", 31)) == 1
+    p.check()
