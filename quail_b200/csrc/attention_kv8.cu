@@ -1,5 +1,5 @@
 // Attention over the 8-bit paged KV cache (kv8.cuh), any head geometry: mma.sync tiles. head_dim 128 with a
-// multiple of 4 query heads per KV head goes to the tcgen05 kernel (a 16k-token chunk: 187 us there, 648 here).
+// multiple of 4 query heads per KV head goes to the tcgen05 kernel (a 16k-token chunk: 192 us there, 648 here).
 //
 // For a row with query q over its visible keys, with codes ck, cv and the
 // exponents ek, ev of their blocks of 16 tokens:

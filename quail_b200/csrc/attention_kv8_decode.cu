@@ -17,7 +17,7 @@
 //     padding. Which of a row's columns is the k-th of a product is free as
 //     long as both operands agree, so a lane takes 16 contiguous codes of a
 //     key for K and of four keys for V and pairs them with byte permutes: no
-//     transposing load. P^T comes out of S^T by movmatrix.
+//     transposing load. P^T comes out of S^T by movmatrix, rounded to bf16 (the sum of p is taken before that).
 //   * Codes become 16-bit numbers in integer instructions, and the integer
 //     pipe, which runs at half rate, is what is scarce: 3 of them for 4 int8
 //     codes of K as f16, 4 for V as bf16 (kv8.cuh). K may be f16 because q,

@@ -298,7 +298,7 @@ struct CopyPool {
   int64_t outer_stride;    // bytes between two layers' (or K's and V's) pools
   int64_t first_block;     // of the launch's blocks
   int outer;               // layers x 2
-  int unit;                // bytes one thread moves at a time: 16, 8, 4, 2 or 1
+  int unit;                // bytes one thread moves at a time: 16, 4 or 1
 };
 struct CopyArgs {
   CopyPool pool[kMaxPools];

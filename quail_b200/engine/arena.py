@@ -23,6 +23,11 @@ Forking and compacting. `fork` starts a key as a copy of another one's first
 tokens: whole pages are shared (each owner holds them), only the page the
 tokens end in is copied, so several continuations of one prompt cost a page
 each. A key that goes back into shared pages takes its own first (`unshare`).
+In an 8-bit arena a token shares its exponent with the 16-token block it is
+in: a key forked from, or rewound to, the middle of a block keeps the exponent
+that the tokens dropped there had grown (and the mark, if one was not finite).
+Where that matters, fork at the parent's end or at a multiple of 16, and give
+tokens that will be dropped a key of their own, as the engine's regions do.
 `compact` moves the held pages to the lowest page numbers. The accounting is
 PagePool's; KVArena's methods of the same names also copy the pages, in every
 layer with one launch (ops.kv_copy_pages), ordered on the current stream

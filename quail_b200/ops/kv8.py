@@ -2,13 +2,15 @@
 
 A layer's K (or V) is a `Pages8`: `codes` [pages, KH, P, D] int8 or e4m3 and
 `bytes` [pages, KH, P / 16] uint8; a value is code * 2^(byte - 127). Half the
-memory of the bf16 arena (a byte and 1/128 of one per value at head_dim 128
+memory of the bf16 arena (a byte and 1/2048 of one per value at head_dim 128
 against two), so twice the documents stay resident, and decode attention
 reads half the bytes. int8 codes keep 7 bits under a block's largest value;
 e4m3 codes keep 4 significant bits of every value, which suits keys with a few
 very wide channels.
 
-Kernels: csrc/kv8_cache.cu, csrc/attention_kv8.cu. Sequence tables, blocks,
+Kernels: csrc/kv8_cache.cu (write, read, page copies), csrc/attention_kv8_tc.cu
+and csrc/attention_kv8.cu (prefill), csrc/attention_kv8_decode.cu; layout and
+conversions in csrc/kv8.cuh. Sequence tables, blocks,
 dseqs and page lists are those of the bf16 attentions (engine/chunk.py).
 """
 
@@ -189,7 +191,9 @@ def _row_numbers(n: int, device) -> torch.Tensor:
 def qk_norm_rope_kv8(qkv, positions, q_norm_w, k_norm_w, cos_sin, slots, k_pages: Pages8, v_pages: Pages8,
                      num_q_heads: int, num_kv_heads: int, eps: float):
     """ops.qk_norm_rope_kv into 8-bit pages (head_dim 128): per-head q/k RMSNorm and NeoX RoPE, q returned
-    as [T, QH, 128]; k and v rows (bf16) quantized into the slots' blocks."""
+    as [T, QH, 128]; k and v rows (bf16) quantized into the slots' blocks. An fp8 model's Q, K and V come
+    here rounded to bf16, which its GEMM's fused epilogue (for bf16 pages) norms and rotates in fp32: a
+    block's exponent needs all its rows, so K and V cannot be written from that epilogue."""
     T = qkv.shape[0]
     q = torch.empty(T, num_q_heads, 128, dtype=torch.bfloat16, device=qkv.device)
     # k and v as pages of one token each, row t in page t, then into the cache
