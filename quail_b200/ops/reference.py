@@ -166,8 +166,7 @@ def kv8_write(x: torch.Tensor, slots: torch.Tensor, codes: torch.Tensor, byte: t
         offs = [sl[i] % 16 for i in kept]
         page, at = blk // (P // 16), blk % (P // 16)
         new = x[kept].float().permute(1, 0, 2)                        # [KH, n, D]
-        b = kv8_byte(new.abs().amax(dim=(1, 2)) if not torch.isnan(new).any() else
-                     new.abs().nan_to_num(float("inf")).amax(dim=(1, 2)), codes.dtype)
+        b = kv8_byte(torch.where(torch.isnan(new), float("inf"), new.abs()).amax(dim=(1, 2)), codes.dtype)
         if min(offs) > 0:
             old = byte[page, :, at].long()
             b = torch.maximum(b, old)

@@ -61,3 +61,12 @@ def test_unshare_refuses_a_place_the_key_does_not_have():
         p.check()
     assert len(p.unshare("c", 31)) == 1
     p.check()
+
+
+@pytest.mark.parametrize("kind", ["int8", "fp8"])
+def test_infinity_beside_nan_marks_its_block_too(kind):
+    p = Pages8.zeros(1, 16, 3, 64, KV8_DTYPES[kind], "cpu")
+    rows = torch.ones(4, 3, 64)
+    rows[1, 0, 5], rows[2, 1, 6] = float("nan"), float("-inf")
+    ref.kv8_write(rows, torch.arange(4, dtype=torch.int32), p.codes, p.bytes)
+    assert p.bytes[0, :, 0].tolist() == [255, 255, 121 if kind == "int8" else 119]
