@@ -137,14 +137,14 @@ def prefill_attention_kv8(q, k_pages: Pages8, v_pages: Pages8, seqs, blocks, pag
 def _few_keys(rows: int, listed: int, page_tokens: int, max_keys: int | None) -> bool:
     """Whether no row of a decode has many keys, by what the host knows.
 
-    Without `max_keys`, by the page list: every other row has a page of its own in it, so one row
-    reads the rest of it at most. That bound is several times what most rows have, so it may be
-    four times as large: the worst case, one row of 4000 keys among short ones, takes 49 us for
-    26, while 8 to 30 short rows take 11 to 20 us for 19 to 27.
+    Without `max_keys`, by the page list: the rows' average, and what one row can have of it, as
+    every other row has a page of its own there. That bound is several times what most rows have,
+    so it may be six times as large: the worst case, one row of 5900 keys among short ones, takes
+    67 us for 26, while 4 to 40 rows of 60 to 250 keys take 10 to 19 us for 17 to 27.
     """
     if max_keys is not None:
         return max_keys <= KV8_FEW_KEYS
-    return (listed - rows + 1) * page_tokens <= 4 * KV8_FEW_KEYS
+    return listed <= rows * KV8_FEW_KEYS // page_tokens and (listed - rows + 1) * page_tokens <= 6 * KV8_FEW_KEYS
 
 
 def decode_attention_kv8(q, k_pages: Pages8, v_pages: Pages8, seqs, dseqs, page_list, softmax_scale: float, *,

@@ -15,7 +15,9 @@ def test_the_rule_goes_by_the_longest_row():
     assert not _few_keys(55, 54 + -(-20000 // 128), 128, None)
     # one long shared document, listed once for all its readers
     assert not _few_keys(8, 8 + -(-7000 // 128), 128, None)
-    assert _few_keys(8, 8 * 2 + 1, 128, None) and _few_keys(30, 30 * 7, 16, None)
+    assert _few_keys(8, 8 * 2 + 1, 128, None) and _few_keys(30, 30 * 7, 16, None) and _few_keys(40, 40 * 2, 128, None)
+    # one row: its keys are the list's
+    assert _few_keys(1, 8, 128, None) and not _few_keys(1, 9, 128, None)
 
 
 def test_a_chunk_carries_the_most_keys_of_its_one_token_rows():
